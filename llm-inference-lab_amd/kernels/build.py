@@ -2,7 +2,8 @@
 
 Kinds of library: ``core`` (embedding, norms, rotary + cache write, matrix
 products, sampling), ``attn_d<D>`` (attention for head size D; one per head
-size that a model needs), ``windowed_attention``, ``linear_attention``, ``gated_recurrence``, ``routed_experts`` and ``stream_ops`` (parts whose
+size that a model needs) and ``e4m3_attn_d<D>`` (the same over a cache of 8 bits), ``e4m3_cache`` (such a cache's write
+and reading), ``verification`` (drafted tokens against the target's distributions), ``windowed_attention``, ``linear_attention``, ``gated_recurrence``, ``routed_experts`` and ``stream_ops`` (parts whose
 sizes are run-time arguments; built when a model names them); beside them ``measure`` (stream and matrix-instruction loops for
 the benchmark's measured peaks) and the plain C++ references of the same operations,
 built with the host compiler for the tests.  A library's file name carries a hash of its sources
@@ -29,6 +30,7 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
 CORE_SOURCES = ("elementwise.hip", "gemm.hip", "decode.hip", "sampling.hip")
 ATTENTION_SOURCE = "attention.hip"
+E4M3_ATTENTION_SOURCE = "e4m3_attention.hip"
 HEADERS = ("common.h",)
 CORE_HEADERS = ("no_alloc.h",)      # included by the core sources only
 FLAGS = ("-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}",
@@ -141,10 +143,21 @@ def attention_library(head_dim: int, force: bool = False) -> str:
     return _compile(f"attn_d{head_dim}", (ATTENTION_SOURCE,), (f"-DHEAD_DIM={head_dim}",), force)
 
 
+def e4m3_attention_library(head_dim: int, force: bool = False) -> str:
+    """Attention over a paged cache of 8-bit keys and values, for one head size."""
+    if head_dim % 16 != 0 or not 16 <= head_dim <= 256:
+        from ..config.errors import UnsupportedSizeError
+        raise UnsupportedSizeError(
+            f"attention kernels take head sizes that are multiples of 16 from 16 to 256, "
+            f"got {head_dim}")
+    return _compile(f"e4m3_attn_d{head_dim}", (E4M3_ATTENTION_SOURCE,), (f"-DHEAD_DIM={head_dim}",), force)
+
+
 # Parts with run-time sizes: one library each, whatever the sizes of the model.
 MIXER_SOURCES = {"windowed_attention": "windowed_attention.hip", "linear_attention": "linear_attention.hip",
                  "routed_experts": "routed_experts.hip", "stream_ops": "stream_ops.hip",
-                 "gated_recurrence": "gated_recurrence.hip"}
+                 "gated_recurrence": "gated_recurrence.hip", "e4m3_cache": "e4m3_cache.hip",
+                 "verification": "verification.hip"}
 
 
 def mixer_library(kind: str, force: bool = False) -> str:
@@ -155,7 +168,8 @@ def mixer_library(kind: str, force: bool = False) -> str:
     feed-forward of many experts of which a row uses a few (choice, sorting, grouped products);
     ``stream_ops``: what lies around the sublayers of a layer (an embedding with hashed token pairs, a
     short causal convolution with per-request state, a token shift, norms of results summed into the
-    stream, a cubic of normed powers, a gated sum into the stream, a soft cap)."""
+    stream, a cubic of normed powers, a gated sum into the stream, a soft cap); ``e4m3_cache``: the write
+    of 8-bit keys and values and their reading; ``verification``: drafted tokens against the target's distributions."""
     return _compile(kind, (MIXER_SOURCES[kind],), (), force)
 
 
@@ -207,11 +221,14 @@ def reference_library(force: bool = False) -> str:
 def library(kind: str, parameter=None, force: bool = False) -> str:
     """The library a part names in ``kernel_libraries()``: ``("core", None)`` or
     ``("attention", head_dim)``, ``("windowed_attention", None)``, ``("linear_attention", None)``,
-    ``("routed_experts", None)``, ``("stream_ops", None)``, ``("gated_recurrence", None)``."""
+    ``("routed_experts", None)``, ``("stream_ops", None)``, ``("gated_recurrence", None)``,
+    ``("e4m3_attention", head_dim)``, ``("e4m3_cache", None)``, ``("verification", None)``."""
     if kind == "core":
         return core_library(force)
     if kind == "attention":
         return attention_library(int(parameter), force)
+    if kind == "e4m3_attention":
+        return e4m3_attention_library(int(parameter), force)
     if kind in MIXER_SOURCES:
         return mixer_library(kind, force)
     raise ValueError(f"no kernel library of kind '{kind}'")
@@ -222,6 +239,7 @@ def build_all(head_dims: Sequence[int] = DEFAULT_HEAD_DIMS, force: bool = True) 
     out = {"core": core_library(force)}
     for d in head_dims:
         out[f"attn_d{d}"] = attention_library(d, force)
+        out[f"e4m3_attn_d{d}"] = e4m3_attention_library(d, force)
     for kind in MIXER_SOURCES:
         out[kind] = mixer_library(kind, force)
     out["measure"] = measure_library(force)

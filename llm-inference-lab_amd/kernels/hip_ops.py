@@ -176,6 +176,28 @@ class AttentionCall:
         self.ops._call(self.lib.llmlab_paged_attention, *a, lib=self.lib)
 
 
+class E4m3AttentionCall:
+    """An attention call over 8-bit keys and values with its unchanging arguments checked and laid out
+    (``HipOps.prepare_attention_e4m3``)."""
+
+    __slots__ = ("ops", "lib", "args", "most_requests", "most_context")
+    REQS, MAX_Q, MAX_CTX, STREAM = 15, 16, 17, -1
+
+    def __init__(self, ops, lib, args, most_requests, most_context):
+        self.ops, self.lib, self.args = ops, lib, args
+        self.most_requests, self.most_context = most_requests, most_context
+
+    def launch(self, n_reqs: int, max_q_len: int, max_ctx_len: int) -> None:
+        if not 0 <= n_reqs <= self.most_requests:
+            raise ValueError("attention: request arrays are shorter than the number of requests")
+        if max_ctx_len > self.most_context:
+            raise ValueError("attention: the block table is too narrow for the longest context")
+        a = self.args
+        a[self.REQS], a[self.MAX_Q], a[self.MAX_CTX] = n_reqs, max_q_len, max_ctx_len
+        a[self.STREAM] = self.ops._stream()
+        self.ops._call(self.lib.llmlab_paged_attention_e4m3, *a, lib=self.lib)
+
+
 class HipOps:
     WORKSPACE_FLOATS = 16 * 1024 * 1024      # 64 MiB of float32 scratch (split partial sums)
     ARRIVED_INTS = 64 * 1024                 # arrival counters: one per (request, kv head) of a step
@@ -196,6 +218,7 @@ class HipOps:
         if self._core.llmlab_abi_version() != 11:
             raise RuntimeError("kernel library and Python bindings disagree on the interface")
         self._attn: Dict[int, ctypes.CDLL] = {}
+        self._e4m3_attn: Dict[int, ctypes.CDLL] = {}
         self._mixer_libs: Dict[str, ctypes.CDLL] = {}
         self._shared: Dict[int, tuple] = {}
         self.num_cus = int(torch.cuda.get_device_properties(self.device).multi_processor_count)
@@ -1079,6 +1102,159 @@ class HipOps:
                              most_context=block_table.shape[1] * page_size, row_req=self._ptr(row_req),
                              heads=(num_heads, num_kv_heads), dtype=qkv.dtype)
 
+    # --------------------------------------- a cache of 8-bit keys and values
+    def _e4m3_attention_lib(self, head_dim: int) -> ctypes.CDLL:
+        lib = self._e4m3_attn.get(head_dim)
+        if lib is None:
+            lib = self._load(build.e4m3_attention_library(head_dim))
+            lib.llmlab_last_error.restype = ctypes.c_char_p
+            lib.llmlab_attention_head_dim.restype = _c_int
+            if lib.llmlab_attention_head_dim() != head_dim:
+                raise RuntimeError(f"attention library for head size {head_dim} reports "
+                                   f"{lib.llmlab_attention_head_dim()}")
+            lib.llmlab_paged_attention_e4m3.argtypes = [
+                _c_ptr, _c_int, _c_long, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int,
+                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_long, _c_int, _c_ptr]
+            lib.llmlab_paged_attention_e4m3.restype = _c_int
+            self._e4m3_attn[head_dim] = lib
+            self.loaded_libraries.append(lib._name)
+        return lib
+
+    def check_e4m3_attention_sizes(self, num_heads: int, num_kv_heads: int, head_dim: int, dtype) -> None:
+        if head_dim % 16 != 0 or not 16 <= head_dim <= 256:
+            raise UnsupportedSizeError(f"attention kernels take head sizes that are multiples of 16 from 16 to 256, "
+                                       f"got {head_dim}")
+        if num_heads % num_kv_heads != 0:
+            raise UnsupportedSizeError(f"{num_heads} heads are not a multiple of {num_kv_heads} kv heads")
+        self._e4m3_attention_lib(head_dim)
+        self._mixer_lib("e4m3_cache")
+
+    def _e4m3_pages(self, what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table) -> None:
+        if page_size < 16 or page_size & (page_size - 1):
+            raise UnsupportedSizeError(f"page size {page_size} is not a power of two >= 16")
+        if head_dim % 16 or not 16 <= head_dim <= 256:
+            raise UnsupportedSizeError(f"{what}: head sizes are multiples of 16 from 16 to 256, got {head_dim}")
+        pages = k_cache.shape[0]
+        for t, name, dtype, shape in ((k_cache, "keys", torch.float8_e4m3fn, (pages, num_kv_heads, page_size, head_dim)),
+                                      (v_cache, "values", torch.float8_e4m3fn, (pages, num_kv_heads, head_dim, page_size)),
+                                      (kv_scale, "scales", torch.uint8, (pages, num_kv_heads, 2, page_size))):
+            self._need(t, f"{what}: cached {name}", dtype)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{what}: cached {name} {tuple(t.shape)} do not have the paged layout {shape}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{what}: cached {name} are not aligned to 16 bytes")
+        self._need(block_table, "block table", torch.int32, contiguous=False)
+        if block_table.dim() != 2 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+            raise ValueError(f"{what}: the block table has a row of page numbers per request")
+
+    def _rows_of(self, what, positions, row_req, rows) -> None:
+        self._need(positions, "positions", torch.int32)
+        self._need(row_req, "row -> request map", torch.int32)
+        if positions.numel() < rows or row_req.numel() < rows:
+            raise ValueError(f"{what}: one position and one request index per row")
+
+    def rope_kv_write_e4m3(self, qkv, num_heads, num_kv_heads, head_dim, inv_freq, positions, row_req, block_table, page_size,
+                           k_cache, v_cache, kv_scale, q_out) -> None:
+        """``rope_kv_write`` for a cache of 8 bits: the query and key heads of ``qkv [rows, (heads + 2 kv_heads) * d]``
+        (bfloat16 or float32) are turned by their row's position (``inv_freq [d / 2]``; None: not turned), the queries
+        go to ``q_out [rows, heads * d]`` (the same dtype; it may be ``qkv``'s own query columns), and every row's keys
+        and values are quantised and stored at its position.
+
+        A key (or value) of ``d`` numbers is stored as ``d`` e4m3 codes and a byte ``e + 127``, ``e`` the smallest whole
+        number from -100 on with ``max |x| <= 448 * 2^e``: ``code = e4m3(x / 2^e)``, ties to even, of the turned
+        number in 64 bits.  What is not finite becomes the code that is not a number, beside the finite ones' scale.
+        Pages: ``k_cache [pages, kv_heads, P, d]`` and ``v_cache [pages, kv_heads, d, P]`` float8_e4m3fn in the order of
+        ``cache/layout.py``, ``kv_scale [pages, kv_heads, 2, P]`` uint8 (keys, then values).  A row whose position
+        has no page in its request's row of the table stores nothing.  Two rows of one call may not name the same position of
+        the same request."""
+        what = "rope_kv_write_e4m3"
+        _dt(qkv)
+        self._need(qkv, "qkv", contiguous=False)
+        rows = qkv.shape[0]
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
+            raise ValueError(f"{what}: qkv {tuple(qkv.shape)} does not hold {num_heads}+2*{num_kv_heads} heads of {head_dim}")
+        self._need(q_out, "queries", qkv.dtype, contiguous=False)
+        if tuple(q_out.shape) != (rows, num_heads * head_dim) or q_out.stride(1) != 1:
+            raise ValueError(f"{what}: queries {tuple(q_out.shape)} for {rows} rows of {num_heads} heads of {head_dim}")
+        self._rows_of(what, positions, row_req, rows)
+        if inv_freq is not None:
+            self._need(inv_freq, "rotary frequencies", torch.float32)
+            if inv_freq.numel() != head_dim // 2:
+                raise ValueError(f"{what}: the frequency table must hold head_dim/2 entries")
+        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+        lib = self._mixer_lib("e4m3_cache")
+        self._call(lib.llmlab_rope_kv_write_e4m3, self._ptr(qkv), _dt(qkv), rows, qkv.stride(0) if rows > 1 else qkv.shape[1],
+                   num_heads, num_kv_heads, head_dim, self._ptr(inv_freq), self._ptr(positions), self._ptr(row_req),
+                   self._ptr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], page_size,
+                   k_cache.shape[0], self._ptr(k_cache), self._ptr(v_cache), self._ptr(kv_scale), self._ptr(q_out),
+                   q_out.stride(0) if rows > 1 else q_out.shape[1], self._stream(), lib=lib)
+
+    def read_kv_e4m3(self, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, positions, row_req, block_table, page_size,
+                     k_out, v_out) -> None:
+        """The stored keys and values of any list of (request, position): row ``i`` of ``k_out`` and ``v_out [rows, kv_heads *
+        d]`` (both bfloat16 or both float32; exact in either) is what the cache holds for position ``positions[i]`` of the
+        request in row ``row_req[i]`` of the table; zeros where that position has no page."""
+        what = "read_kv_e4m3"
+        rows = k_out.shape[0]
+        _dt(k_out)
+        self._need(k_out, "keys read back")
+        self._need(v_out, "values read back", k_out.dtype)
+        for t in (k_out, v_out):
+            if tuple(t.shape) != (rows, num_kv_heads * head_dim):
+                raise ValueError(f"{what}: output {tuple(t.shape)} for {rows} rows of {num_kv_heads} heads of {head_dim}")
+        self._rows_of(what, positions, row_req, rows)
+        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+        lib = self._mixer_lib("e4m3_cache")
+        self._call(lib.llmlab_read_kv_e4m3, self._ptr(k_cache), self._ptr(v_cache), self._ptr(kv_scale), num_kv_heads, head_dim,
+                   rows, self._ptr(positions), self._ptr(row_req), self._ptr(block_table), block_table.stride(0),
+                   block_table.shape[1], block_table.shape[0], page_size, k_cache.shape[0], self._ptr(k_out), self._ptr(v_out),
+                   _dt(k_out), self._stream(), lib=lib)
+
+    def paged_attention_e4m3(self, q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
+                             q_start, start_pos, n_reqs, max_q_len, max_ctx_len, window, scale, out) -> None:
+        """``paged_attention`` over a cache of 8 bits (``rope_kv_write_e4m3``): request ``b < n_reqs`` brings the rows
+        ``q_start[b] .. q_start[b + 1] - 1`` of ``q [rows, >= heads * d]`` (one token, a few, or a portion of a prompt;
+        none: nothing is done) at the positions from ``start_pos[b]`` on, whose keys and values are already stored; the row at
+        position p sees the keys ``max(0, p - window + 1) .. p`` (``window`` None: from 0 on).  Keys whose page the
+        table does not have are not seen, and a row that sees none gives zeros.  ``q`` and ``out [rows, heads * d]`` are
+        both bfloat16 or both float32 (products in 24 bits); scores, softmax and sums are float32.  ``max_q_len`` and
+        ``max_ctx_len`` are the longest portion and context among the requests.  Rows behind the last request keep what they
+        hold."""
+        self.prepare_attention_e4m3(q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
+                                    q_start, start_pos, window, scale, out).launch(n_reqs, max_q_len, max_ctx_len)
+
+    def prepare_attention_e4m3(self, q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
+                               q_start, start_pos, window, scale, out) -> "E4m3AttentionCall":
+        """What of such a call does not change while the same buffers serve the same number of rows, checked and laid out once
+        (as ``prepare_attention``)."""
+        what = "attention"
+        if num_kv_heads <= 0 or num_heads % num_kv_heads:
+            raise UnsupportedSizeError(f"{num_heads} heads are not a multiple of {num_kv_heads} kv heads")
+        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+        lib = self._e4m3_attention_lib(head_dim)
+        _dt(q)
+        rows = q.shape[0]
+        self._need(q, "queries", contiguous=False)
+        self._need(out, "attention output", q.dtype)
+        self._need(q_start, "request row starts", torch.int32)
+        self._need(start_pos, "request start positions", torch.int32)
+        if q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1) or q.shape[1] < num_heads * head_dim:
+            raise ValueError("attention: the query rows are too narrow")
+        if tuple(out.shape) != (rows, num_heads * head_dim):
+            raise ValueError(f"attention: output {tuple(out.shape)} != ({rows}, {num_heads * head_dim})")
+        q_stride = q.stride(0) if rows > 1 else q.shape[1]
+        if q.data_ptr() % 16 or out.data_ptr() % 16 or q_stride * q.element_size() % 16:
+            raise ValueError("attention: queries and output are not aligned to 16 bytes")
+        if window is not None and window <= 0:
+            raise ValueError(f"attention: a window holds at least the current position, got {window}")
+        args = [self._ptr(q), _dt(q), q_stride, num_heads, num_kv_heads, self._ptr(k_cache), self._ptr(v_cache),
+                self._ptr(kv_scale), k_cache.shape[0], self._ptr(block_table), block_table.stride(0), block_table.shape[1],
+                page_size, self._ptr(q_start), self._ptr(start_pos), 0, 0, 0, int(window) if window else 0, float(scale),
+                self._ptr(out), num_heads * head_dim, rows, None]
+        return E4m3AttentionCall(self, lib, args,
+                                 most_requests=min(q_start.numel() - 1, start_pos.numel(), block_table.shape[0]),
+                                 most_context=block_table.shape[1] * page_size)
+
     # ------------------------------------------- layer norm, plain activations
     def layernorm(self, x, weight, eps, out, rows=None) -> None:
         """``out[i] = (x[r] - mean) / sqrt(var + eps) * weight`` for ``r = rows[i]`` (all rows in
@@ -1176,6 +1352,20 @@ class HipOps:
         if lib is None:
             lib = self._load(build.mixer_library(kind))
             lib.llmlab_last_error.restype = ctypes.c_char_p
+            if kind == "e4m3_cache":
+                lib.llmlab_rope_kv_write_e4m3.argtypes = [
+                    _c_ptr, _c_int, _c_int, _c_size, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                    _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]
+                lib.llmlab_rope_kv_write_e4m3.restype = _c_int
+                lib.llmlab_read_kv_e4m3.argtypes = [
+                    _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                    _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr]
+                lib.llmlab_read_kv_e4m3.restype = _c_int
+            if kind == "verification":
+                lib.llmlab_verify_drafts.argtypes = [
+                    _c_ptr, _c_size, _c_ptr, _c_size, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr,
+                    _c_ptr, _c_size, _c_ptr]
+                lib.llmlab_verify_drafts.restype = _c_int
             if kind == "windowed_attention":
                 lib.llmlab_project_norm_write.argtypes = [
                     _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr,
@@ -2575,3 +2765,44 @@ class HipOps:
         self._call(self._core.llmlab_sample,
             self._ptr(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab,
             self._ptr(temperatures), self._ptr(uniforms), self._ptr(out), self._stream())
+
+    def verify_drafts(self, logits, draft_logits, drafts, row_start, temperatures, uniforms, accepted, tokens) -> None:
+        """Speculative decoding's check: which drafted tokens stand, and the token behind them.
+
+        Request ``b`` of ``n`` has the rows ``row_start[b] .. row_start[b + 1] - 1`` of ``logits [rows, vocab]`` (float32), at
+        least one: one for each of its drafted tokens and one more.  Its drafted token ``j`` is number ``row_start[b] - b +
+        j`` of ``drafts [rows - n]``, and so is that token's row of ``draft_logits`` (float32 ``[rows - n, vocab]``, or
+        None: every draft is a certain guess).  With ``p_j`` the softmax of row ``j`` over the request's temperature and
+        ``q_j`` that of the draft's logits, token ``j`` stands while ``uniforms[row_start[b] + j] * q_j(token) <
+        p_j(token)``.  At the first that falls the next token is drawn from ``max(p_j - q_j, 0)``, behind the last from the
+        last row's ``p``: the first token at which the running sum reaches ``uniforms[row_start[b + 1] - 1]`` times
+        the whole.  Temperature 0: a token stands while it is its row's argmax (the smallest index among equals), and the
+        next token is the argmax of the row that is reached.  ``accepted[b]`` is how many stand, ``tokens[b]`` the
+        next token, -1 where its row is no distribution.  A logit that is not a number counts as minus infinity, a drafted
+        token outside the vocabulary falls.  ``uniforms [rows]`` are in [0, 1).  The kernel set's workspace is used:
+        calls of one kernel set go to one stream at a time."""
+        what = "verify_drafts"
+        self._need(logits, "logits", torch.float32, contiguous=False)
+        if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+            raise ValueError(f"{what}: logits rows must be contiguous")
+        rows, vocab = logits.shape
+        for t, name, dtype in ((drafts, "drafted tokens", torch.int32), (row_start, "request row starts", torch.int32),
+                               (temperatures, "temperatures", torch.float32), (uniforms, "uniform numbers", torch.float32),
+                               (accepted, "accepted counts", torch.int32), (tokens, "next tokens", torch.int32)):
+            self._need(t, name, dtype)
+        n = row_start.numel() - 1
+        if n < 0 or rows < n or drafts.numel() < rows - n or uniforms.numel() < rows:
+            raise ValueError(f"{what}: {n} requests with {rows} rows of logits need {rows - n} drafted tokens and {rows} uniform numbers")
+        if min(temperatures.numel(), accepted.numel(), tokens.numel()) < n:
+            raise ValueError(f"{what}: one temperature, one count and one token per request")
+        if draft_logits is not None:
+            self._need(draft_logits, "draft logits", torch.float32, contiguous=False)
+            if tuple(draft_logits.shape) != (rows - n, vocab) or (draft_logits.stride(1) != 1 and vocab > 1):
+                raise ValueError(f"{what}: draft logits {tuple(draft_logits.shape)} != ({rows - n}, {vocab})")
+        if rows + (rows - n if draft_logits is not None else 0) > 65535:
+            raise UnsupportedSizeError(f"{what}: at most 65535 rows of logits in one call, got {rows} of the target's")
+        lib = self._mixer_lib("verification")
+        self._call(lib.llmlab_verify_drafts, self._ptr(logits), logits.stride(0) if rows > 1 else vocab, self._ptr(draft_logits),
+                   draft_logits.stride(0) if draft_logits is not None and rows - n > 1 else vocab, self._ptr(drafts),
+                   self._ptr(row_start), self._ptr(temperatures), self._ptr(uniforms), n, rows, vocab, self._ptr(accepted),
+                   self._ptr(tokens), self._ptr(self.workspace), self.workspace.numel() * 4, self._stream(), lib=lib)
