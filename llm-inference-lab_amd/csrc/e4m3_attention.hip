@@ -64,9 +64,20 @@ struct Args {
   void* out;                   // [rows, out_stride]
   long q_stride, out_stride;
   int table_stride, table_width, page_shift, pages;
-  int nq, nkv, window, rows;
+  int nq, nkv, window, rows, reqs, splits;
   float scale2;                // the scores' factor times log2 e
+  float* o_part;               // [rows * nq, splits, D]    (splits > 1)
+  float* ml_part;              // [rows * nq, splits, 2]
 };
+
+// Four numbers of a row's output: its sums over the sum of its probabilities, zero where it saw no key.
+template <typename T>
+__device__ __forceinline__ void write_output(const Args& a, int row, int head, int i, floatx4 sum, float weight) {
+  T* out = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + i;
+  const bool any = weight > 0.f || weight != weight;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = from_float<T>(any ? sum[j] / weight : 0.f);
+}
 
 template <typename T>
 constexpr int parts_of() { return std::is_same<T, float>::value ? 3 : 1; }
@@ -83,212 +94,390 @@ __device__ __forceinline__ void split(float x, bf16_t (&part)[PARTS]) {
 
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
-// The block's waves share 16 rows (a row: a token and a head of the group that shares a kv head) and split their keys in
-// steps of 32; the waves' sums meet in LDS.
-constexpr int WAVES = 4;
-template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void attention_e4m3_kernel(Args a) {
-  constexpr int PARTS = parts_of<T>();
-  __shared__ float s_o[WAVES][16][D + 4];
-  __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv;
-  const int r0 = a.q_start[b], count = a.q_start[b + 1] - r0, before = a.start_pos[b];
-  const int total = count * G, row0 = blockIdx.x * 16;
-  if (row0 >= total || r0 < 0 || count > a.rows - r0) return;
-  const int last = min(row0 + 16, total) - 1;
-  const int P = 1 << a.page_shift;
+// What a step of 32 keys reads: of each of its two blocks of 16 keys the codes of the keys and values and their scales'
+// bytes (a lane's key's, and those of its four values).
+struct Step {
+  uint4v k[2][KP];
+  unsigned v[2][DB];      // a word: the four keys 4 g .. 4 g + 3 of a number
+  unsigned ks[2], vs[2];
+  bool there[2];
+};
 
-  // this lane's row
-  const int row = row0 + c;
-  const bool valid = row < total;
-  const int tok = valid ? row / G : 0, head = kvh * G + (valid ? row % G : 0), pos = before + tok;
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  bf16x8 qf[PARTS][KP][2];
-  const T* q = (const T*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
-#pragma unroll
-  for (int kp = 0; kp < KP; ++kp)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int dd = kp * 64 + g * 16 + h * 8 + i;
-        bf16_t part[PARTS];
-        split<PARTS>(valid && dd < D ? to_float(q[dd]) : 0.f, part);
-#pragma unroll
-        for (int n = 0; n < PARTS; ++n) qf[n][kp][h][i] = part[n];
-      }
+// The rows of one tile as a lane has them (row 16 qb + lane % 16), and what is summed for them so far.
+template <int QB, int PARTS>
+struct Rows {
+  bool valid[QB];
+  int pos[QB], lo[QB];
+  bf16x8 q[QB][PARTS][KP][2];
+  floatx4 o[QB][DB];
+  float m[QB], l[QB];
+};
 
-  // the keys that some row of the tile sees, and this wave's steps among them
-  const int first_pos = before + row0 / G, key_hi = before + last / G;
-  const int key_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
-  const int step_lo = key_lo >> 5, steps = (key_hi >> 5) - step_lo + 1;
-  const int per = (steps + WAVES - 1) / WAVES;
-  const int my_lo = step_lo + wave * per, my_hi = min(my_lo + per, step_lo + steps);
-
-  floatx4 o[DB];
+template <typename T, int QB, int PARTS>
+__device__ __forceinline__ void load_rows(const Args& a, Rows<QB, PARTS>& r, int r0, int before, int kvh, int row0, int total, int c,
+                                          int g) {
+  const int G = a.nq / a.nkv;
 #pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = NEG_INF, l = 0.f;
-
-  for (int step = my_lo; step < my_hi; ++step) {
-    const int kb = step * 32;
-    floatx4 s[2];
-    unsigned vw[2][DB], vs[2];      // the values' codes: a word holds the four keys 4 g .. 4 g + 3 of a number
-    bool there[2];
+  for (int qb = 0; qb < QB; ++qb) {
+    const int row = row0 + qb * 16 + c;
+    r.valid[qb] = row < total;
+    const int tok = r.valid[qb] ? row / G : 0, head = kvh * G + (r.valid[qb] ? row - tok * G : 0);
+    r.pos[qb] = before + tok;
+    r.lo[qb] = a.window > 0 ? max(0, r.pos[qb] - a.window + 1) : 0;
+    const T* q = (const T*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
 #pragma unroll
-    for (int h2 = 0; h2 < 2; ++h2) {
-      const int key = kb + h2 * 16, slot = key >> a.page_shift;
-      const int page = slot < a.table_width && key <= key_hi && key + 15 >= key_lo ? a.table[(size_t)b * a.table_stride + slot] : -1;
-      there[h2] = page >= 0 && page < a.pages;
-      const size_t at = ((size_t)(there[h2] ? page : 0) * a.nkv + kvh) << a.page_shift;
-      const int off = key & (P - 1);
-      const unsigned char* kp = a.k + at * D + (size_t)off * D;
-      const unsigned char* vp = a.v + at * D + (size_t)off * D;
-      const unsigned char* sp = a.scale + 2 * at + off;
-      s[h2] = floatx4{0.f, 0.f, 0.f, 0.f};
-      vs[h2] = 0;
+    for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) vw[h2][db] = 0;
-      if (!there[h2]) continue;
-      const float ks = power_of_byte(sp[c]);
-      vs[h2] = *(const unsigned*)(sp + P + 4 * g);
+      for (int h = 0; h < 2; ++h) {
+        const int dd = kp * 64 + g * 16 + h * 8;
+        const bool in = r.valid[qb] && dd < D;      // (D is a multiple of 16: eight numbers are in or out together)
+        if constexpr (PARTS == 1) {
+          const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+          const bf16x8 x = *(const bf16x8*)(q + (in ? dd : 0));
+          r.q[qb][0][kp][h] = in ? x : zero;
+        } else {
+          const floatx4 x = *(const floatx4*)(q + (in ? dd : 0)), y = *(const floatx4*)(q + (in ? dd + 4 : 4));
 #pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int sixteen = i * 4 + g;      // (past the last: the queries are zero there)
-        const uint4v w = *(const uint4v*)(kp + (size_t)(min(sixteen, D / 16 - 1) * 16 + c) * 16);
-        const bf16x8 k0 = eight_numbers(w[0], w[1], ks), k1 = eight_numbers(w[2], w[3], ks);
+          for (int i = 0; i < 8; ++i) {
+            bf16_t part[PARTS];
+            split<PARTS>(in ? (i < 4 ? x[i & 3] : y[i & 3]) : 0.f, part);
 #pragma unroll
-        for (int n = PARTS - 1; n >= 0; --n) {
-          s[h2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[n][i][0], s[h2], 0, 0, 0);
-          s[h2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[n][i][1], s[h2], 0, 0, 0);
+            for (int n = 0; n < PARTS; ++n) r.q[qb][n][kp][h][i] = part[n];
+          }
         }
       }
+    r.m[qb] = NEG_INF;
+    r.l[qb] = 0.f;
 #pragma unroll
-      for (int vg = 0; vg < VG; ++vg) {
-        constexpr int FULL = 4;
-        const int wide = DB - 4 * vg < FULL ? DB - 4 * vg : FULL;
-        const unsigned* wp = (const unsigned*)(vp + vg * 1024 + (size_t)(g * 16 + c) * wide * 4);
+    for (int db = 0; db < DB; ++db) r.o[qb][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  The running
+// maximum is kept in the units of the exponent and is raised only when a score exceeds it by more than LAZY_MAX: until then p may
+// be as large as 2^8, which float32 sums and bfloat16 probabilities hold without loss, and rescaling the sums is rare.
+template <bool MASKED, int QB, int PARTS>
+__device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step& f, int kb, int g) {
+  floatx4 s[2][QB];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (vg * 4 + j < DB) vw[h2][vg * 4 + j] = wp[j];
-      }
+  for (int h2 = 0; h2 < 2; ++h2) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) s[h2][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const float ks = power_of_byte(f.ks[h2]);
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const uint4v w = f.k[h2][i];
+      const bf16x8 k0 = eight_numbers(w[0], w[1], ks), k1 = eight_numbers(w[2], w[3], ks);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int n = PARTS - 1; n >= 0; --n) {
+          s[h2][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[qb][n][i][0], s[h2][qb], 0, 0, 0);
+          s[h2][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[qb][n][i][1], s[h2][qb], 0, 0, 0);
+        }
     }
-    const bool masked = !(there[0] && there[1] && kb + 31 <= first_pos && (a.window <= 0 || kb >= key_hi - a.window + 1));
+  }
+  float vs[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) vs[i] = power_of_byte((f.vs[i >> 2] >> (8 * (i & 3))) & 255u);
+  auto key = [&](int i) { return kb + (i >> 2) * 16 + g * 4 + (i & 3); };
+  auto sees = [&](int qb, int i) { return f.there[i >> 2] && r.valid[qb] && key(i) <= r.pos[qb] && key(i) >= r.lo[qb]; };
+  bf16x8 pf[QB][PARTS];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
     float p[8];
-    float mx = NEG_INF;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int j = kb + (i >> 2) * 16 + g * 4 + (i & 3);
-      const bool sees = there[i >> 2] && valid && j <= pos && j >= lo;
-      p[i] = sees ? s[i >> 2][i & 3] * a.scale2 : NEG_INF;
-      mx = fmaxf(mx, p[i]);
+      p[i] = s[i >> 2][qb][i & 3] * a.scale2;
+      if (MASKED && !sees(qb, i)) p[i] = NEG_INF;
     }
+    float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
     mx = max_across_rows(mx);
-    // The maximum is raised only when a score exceeds it by more than LAZY_MAX: until then p may be as large as 2^8,
-    // which float32 sums and bfloat16 probabilities hold without loss, and rescaling the sums is rare.
-    const bool grow = mx > m + LAZY_MAX;
+    const bool grow = mx > r.m[qb] + LAZY_MAX;
     if (__any(grow)) {
-      const float m_new = grow ? mx : m, alpha = grow ? fast_exp2(m - m_new) : 1.f;
-      l *= alpha;
+      const float m_new = grow ? mx : r.m[qb], alpha = grow ? fast_exp2(r.m[qb] - m_new) : 1.f;
+      r.l[qb] *= alpha;
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] *= alpha;
-      m = m_new;
+      for (int db = 0; db < DB; ++db) r.o[qb][db] *= alpha;
+      r.m[qb] = m_new;
     }
-    const float neg_m = m == NEG_INF ? 0.f : -m;      // (no key seen yet: every p is 2^-inf = 0)
-    bf16x8 pf[PARTS];
+    const float neg_m = MASKED && r.m[qb] == NEG_INF ? 0.f : -r.m[qb];      // (no key seen yet: every p is 2^-inf = 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(p[i] + neg_m);
+    r.l[qb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = fast_exp2(p[i] + neg_m);
-      l += p[i];
-      const int j = kb + (i >> 2) * 16 + g * 4 + (i & 3);
-      const bool sees = there[i >> 2] && valid && j <= pos && j >= lo;      // (the scale of another place is not used)
-      const float w = sees ? p[i] * power_of_byte((vs[i >> 2] >> (8 * (i & 3))) & 255u) : 0.f;
+      const float w = MASKED && !sees(qb, i) ? 0.f : p[i] * vs[i];      // (the scale of a place not seen is not used)
       bf16_t part[PARTS];
       split<PARTS>(w, part);
 #pragma unroll
-      for (int n = 0; n < PARTS; ++n) pf[n][i] = part[n];
+      for (int n = 0; n < PARTS; ++n) pf[qb][n][i] = part[n];
     }
-    // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not
-    // keep out of the product: they become zeros, and the rows that do see them become no numbers.
+  }
+  // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not keep
+  // out of the product: they become zeros, and the rows that do see them become no numbers.
+  if constexpr (MASKED) {
     bool strange = false;
-    if (masked) {
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2)
+    for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const unsigned x = vw[h2][db] & 0x7f7f7f7fu;
-          strange |= ((x + 0x01010101u) & 0x80808080u) != 0;
-        }
-      strange = __any(strange);
-    }
-    if (strange) {
-      bf16x8 ind;
+      for (int db = 0; db < DB; ++db) strange |= (((f.v[h2][db] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+    if (__any(strange)) {
+      bf16x8 seen[QB];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = kb + (i >> 2) * 16 + g * 4 + (i & 3);
-        ind[i] = there[i >> 2] && valid && j <= pos && j >= lo ? (bf16_t)1.f : (bf16_t)0.f;
-      }
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) seen[qb][i] = sees(qb, i) ? (bf16_t)1.f : (bf16_t)0.f;
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         bf16x8 bad;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const unsigned shift = 8 * (i & 3);
-          const bool nan = ((vw[i >> 2][db] >> shift) & 0x7fu) == 0x7fu;
+          const bool nan = ((f.v[i >> 2][db] >> shift) & 0x7fu) == 0x7fu;
           bad[i] = nan ? (bf16_t)1.f : (bf16_t)0.f;
-          if (nan) vw[i >> 2][db] &= ~(0xffu << shift);
+          if (nan) f.v[i >> 2][db] &= ~(0xffu << shift);
         }
-        const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, ind, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (hits[i] > 0.f) o[db][i] = __builtin_nanf("");
+        for (int qb = 0; qb < QB; ++qb) {
+          const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, seen[qb], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hits[i] > 0.f) r.o[qb][db][i] = __builtin_nanf("");
+        }
       }
     }
+  }
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      const bf16x8 vf = eight_numbers(vw[0][db], vw[1][db], 1.f);
+  for (int db = 0; db < DB; ++db) {
+    const bf16x8 vf = eight_numbers(f.v[0][db], f.v[1][db], 1.f);
 #pragma unroll
-      for (int n = PARTS - 1; n >= 0; --n) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[db], 0, 0, 0);
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int n = PARTS - 1; n >= 0; --n) r.o[qb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][n], r.o[qb][db], 0, 0, 0);
+  }
+}
+
+// Few rows a request: NW waves share a tile of 16 QB rows (a row: a token and a head of the group that shares a kv head) and
+// split the block's keys in steps of 32; their sums meet in LDS.  The keys of a tile are split over a.splits blocks as
+// well, whose sums a kernel of its own puts together.  Bound by the reading of the codes.
+template <int QB, int NW>
+constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
+
+template <typename T, int QB, int NW>
+__global__ __launch_bounds__(64 * NW) void attention_e4m3_split_kernel(Args a) {
+  constexpr int PARTS = parts_of<T>(), TR = 16 * QB, RS = D + 4;
+  __shared__ __attribute__((aligned(16))) float lds[split_lds_floats<QB, NW>()];
+  float* s_m = lds + NW * TR * RS;
+  float* s_l = s_m + NW * TR;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.z, kvh = blockIdx.y / a.splits, part = blockIdx.y % a.splits, G = a.nq / a.nkv;
+  const int r0 = a.q_start[b], count = a.q_start[b + 1] - r0, before = a.start_pos[b];
+  const int total = count * G, row0 = blockIdx.x * TR;
+  if (row0 >= total || r0 < 0 || count > a.rows - r0) return;
+  const int last = min(row0 + TR, total) - 1;
+  const int P = 1 << a.page_shift;
+  Rows<QB, PARTS> r;
+  load_rows<T, QB, PARTS>(a, r, r0, before, kvh, row0, total, c, g);
+
+  // the keys that some row of the tile sees, this block's steps of 32 among them, and this wave's
+  const int first_pos = before + row0 / G, key_hi = before + last / G;
+  const int key_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
+  const int full_lo = a.window > 0 ? max(0, key_hi - a.window + 1) : 0;      // from here on every row sees a key before first_pos
+  const int step_lo = key_lo >> 5, step_hi = (key_hi >> 5) + 1;
+  const int per = (step_hi - step_lo + a.splits - 1) / a.splits;
+  const int blk_lo = step_lo + part * per, blk_hi = min(blk_lo + per, step_hi);
+  const int per_wave = (max(blk_hi - blk_lo, 0) + NW - 1) / NW;
+  const int my_lo = blk_lo + wave * per_wave, my_hi = min(my_lo + per_wave, blk_hi);
+
+  // The page numbers of up to 32 steps are read ahead, a block of 16 keys a lane; the loads of the next step are in
+  // flight while one is computed.  A page that is not there is read as page 0 and its keys are seen by nobody.
+  for (int base = my_lo; base < my_hi; base += 32) {
+    const int end = min(base + 32, my_hi);
+    int page_v = -1;
+    {
+      const int key = base * 32 + lane * 16, slot = key >> a.page_shift;
+      if (key <= key_hi && key + 15 >= key_lo && slot < a.table_width) page_v = a.table[(size_t)b * a.table_stride + slot];
+      if (page_v >= a.pages) page_v = -1;
+    }
+    auto fetch = [&](int step, Step& f) {
+      const int st = min(step, end - 1);
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        const int page = __builtin_amdgcn_readlane(page_v, (st - base) * 2 + h2);
+        f.there[h2] = page >= 0;
+        const size_t at = ((size_t)max(page, 0) * a.nkv + kvh) << a.page_shift;
+        const int off = (st * 32 + h2 * 16) & (P - 1);
+        const unsigned char* kp = a.k + (at + off) * D + lane * 16;
+        const unsigned char* vp = a.v + (at + off) * D;
+        const unsigned char* sp = a.scale + 2 * at + off;
+#pragma unroll
+        for (int i = 0; i < KP; ++i)      // (a sixteen past the last: the queries are zero there)
+          f.k[h2][i] = *(const uint4v*)(kp + (D % 64 == 0 ? i * 1024 : (min(i * 4 + g, D / 16 - 1) - g) * 256));
+#pragma unroll
+        for (int vg = 0; vg < VG; ++vg) {
+          const int wide = DB - 4 * vg < 4 ? DB - 4 * vg : 4;
+          const unsigned* wp = (const unsigned*)(vp + vg * 1024 + lane * wide * 4);
+          if (wide == 4) {
+            const uint4v w = *(const uint4v*)wp;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (vg * 4 + j < DB) f.v[h2][vg * 4 + j] = w[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (vg * 4 + j < DB) f.v[h2][vg * 4 + j] = wp[j];
+          }
+        }
+        f.ks[h2] = sp[c];
+        f.vs[h2] = *(const unsigned*)(sp + P + 4 * g);
+      }
+    };
+    Step next;
+    fetch(base, next);
+    for (int step = base; step < end; ++step) {
+      Step cur = next;
+      fetch(step + 1, next);
+      __builtin_amdgcn_sched_barrier(0);
+      const int kb = step * 32;
+      if (cur.there[0] && cur.there[1] && kb + 31 <= first_pos && kb >= full_lo)      // (rows past the last are not stored)
+        add_step<false, QB, PARTS>(a, r, cur, kb, g);
+      else
+        add_step<true, QB, PARTS>(a, r, cur, kb, g);
     }
   }
 
   // a row's four lanes hold its keys' sums, every lane the numbers 16 db + 4 g + i of its row
-  l += __shfl_xor(l, 16, WAVE);
-  l += __shfl_xor(l, 32, WAVE);
-  if (g == 0) {
-    s_m[wave][c] = m;
-    s_l[wave][c] = l;
-  }
 #pragma unroll
-  for (int db = 0; db < DB; ++db) *(floatx4*)&s_o[wave][c][db * 16 + g * 4] = o[db];
-  __syncthreads();
-  for (int n = threadIdx.x; n < 16 * D; n += 64 * WAVES) {
-    const int r = n / D, i = n - r * D;
-    if (row0 + r >= total) continue;
-    float top = NEG_INF;
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_m[w][r]);
-    float sum = 0.f, weight = 0.f;
-    for (int w = 0; w < WAVES; ++w) {
-      // (no maximum: no key that the row sees, sums of zero, or scores that are no numbers, and sums likewise)
-      const float f = s_m[w][r] == NEG_INF ? 1.f : fast_exp2(s_m[w][r] - top);
-      sum += f * s_o[w][r][i];
-      weight += f * s_l[w][r];
+  for (int qb = 0; qb < QB; ++qb) {
+    float l = r.l[qb];
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+    if (g == 0) {
+      s_m[wave * TR + qb * 16 + c] = r.m[qb];
+      s_l[wave * TR + qb * 16 + c] = l;
     }
-    const int t = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
-    ((T*)a.out)[(size_t)(r0 + t) * a.out_stride + (size_t)h * D + i] = from_float<T>(weight > 0.f || weight != weight ? sum / weight : 0.f);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) *(floatx4*)&lds[(wave * TR + qb * 16 + c) * RS + db * 16 + g * 4] = r.o[qb][db];
   }
+  __syncthreads();
+  const int rows = last - row0 + 1;
+  for (int n = threadIdx.x; n < rows * (D / 4); n += 64 * NW) {
+    const int row = n / (D / 4), i = (n - row * (D / 4)) * 4;
+    float top = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, s_m[w * TR + row]);
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    float weight = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // (no maximum: no key that the row sees, sums of zero, or scores that are no numbers, and sums likewise)
+      const float m = s_m[w * TR + row], f = m == NEG_INF ? 1.f : fast_exp2(m - top);
+      sum += f * *(const floatx4*)&lds[(w * TR + row) * RS + i];
+      weight += f * s_l[w * TR + row];
+    }
+    const int tok = (row0 + row) / G, head = kvh * G + (row0 + row) - tok * G;
+    const size_t at = (size_t)(r0 + tok) * a.nq + head;
+    if (a.splits > 1) {
+      *(floatx4*)(a.o_part + (at * a.splits + part) * D + i) = sum;
+      if (i == 0) {
+        a.ml_part[(at * a.splits + part) * 2] = top;
+        a.ml_part[(at * a.splits + part) * 2 + 1] = weight;
+      }
+    } else {
+      write_output<T>(a, r0 + tok, head, i, sum, weight);
+    }
+  }
+}
+
+// The splits of a row put together: a wave a (row, head), four numbers a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
+  const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = at / a.nq;
+  if (row < a.q_start[0] || row >= a.q_start[a.reqs] || row >= a.rows) return;
+  const float* ml = a.ml_part + (size_t)at * a.splits * 2;
+  float top = NEG_INF, l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[2 * s]);
+  top = full_wave_max(top);
+  const float* o = a.o_part + (size_t)at * a.splits * D;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  const int i = lane * 4;
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {      // four splits' loads at a time
+    floatx4 x[4];
+    float m[4], w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int s = min(s0 + j, a.splits - 1);
+      m[j] = ml[2 * s];
+      w[j] = ml[2 * s + 1];
+      x[j] = *(const floatx4*)(o + (size_t)s * D + (i < D ? i : 0));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (s0 + j >= a.splits) continue;
+      const float f = m[j] == NEG_INF ? 1.f : fast_exp2(m[j] - top);
+      sum += f * x[j];
+      l += f * w[j];
+    }
+  }
+  if (i < D) write_output<T>(a, row, at - row * a.nq, i, sum, l);
 }
 
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
 extern "C" int llmlab_attention_head_dim() { return D; }
 
+// For measurements and tests: the number of key splits (0: by the rule)
+static int g_force_splits = 0, g_force_waves = 0;
+extern "C" void llmlab_debug_attention_e4m3(int splits, int waves) {
+  g_force_splits = splits;
+  g_force_waves = waves;
+}
+
+// Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys
+// for each of its waves.
+static int key_splits(long blocks, int visible, int num_cus) {
+  if (blocks >= num_cus) return 1;
+  const long steps = (visible + 31) / 32, most = (steps + 7) / 8;
+  return (int)max(1L, min(min(2L * num_cus / blocks, most), 128L));
+}
+
+template <typename T, int QB, int NW>
+static void launch_split_waves(const Args& a, dim3 grid, hipStream_t stream) {
+  hipLaunchKernelGGL((attention_e4m3_split_kernel<T, QB, NW>), grid, dim3(64 * NW), 0, stream, a);
+}
+
+template <typename T, int QB>
+static int launch_split(Args a, long most_rows, int visible, float* workspace, size_t workspace_floats, int num_cus,
+                        hipStream_t stream) {
+  const long tiles = (most_rows + 16 * QB - 1) / (16 * QB);
+  a.splits = g_force_splits > 0 ? g_force_splits : key_splits(tiles * a.nkv * a.reqs, visible, num_cus > 0 ? num_cus : 256);
+  const size_t each = (size_t)a.rows * a.nq * (D + 2);
+  a.splits = (int)max((size_t)1, min((size_t)min(a.splits, 65535 / a.nkv), workspace_floats / max(each, (size_t)1)));
+  if (a.splits > 1) {
+    a.o_part = workspace;
+    a.ml_part = workspace + (size_t)a.rows * a.nq * a.splits * D;
+  }
+  const dim3 grid((unsigned)tiles, a.nkv * a.splits, a.reqs);
+  constexpr int WIDE = split_lds_floats<QB, 8>() * 4 <= 80 * 1024 ? 8 : 4;
+  if (g_force_waves == 8)
+    launch_split_waves<T, QB, WIDE>(a, grid, stream);
+  else
+    launch_split_waves<T, QB, 4>(a, grid, stream);
+  LLMLAB_LAUNCH_CHECK("attention(e4m3)");
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(attention_e4m3_merge_kernel<T>, dim3((unsigned)(((long)a.rows * a.nq + 3) / 4)), dim3(256), 0, stream, a);
+    LLMLAB_LAUNCH_CHECK("attention(e4m3, merge)");
+  }
+  return 0;
+}
+
 extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stride, int nq, int nkv, const void* k, const void* v,
                                            const void* kv_scale, int pages, const int* table, int table_stride, int table_width,
                                            int page_size, const int* q_start, const int* start_pos, int reqs, int max_q_len,
                                            int max_ctx_len, int window, float scale, void* out, long out_stride, int rows,
-                                           hipStream_t stream) {
+                                           float* workspace, size_t workspace_floats, int num_cus, hipStream_t stream) {
   LLMLAB_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && nkv <= 65535, "attention(e4m3): %d heads, %d kv heads", nq, nkv);
   LLMLAB_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "attention(e4m3): page size %d is not a power of two >= 16",
                  page_size);
@@ -300,14 +489,13 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
                  "attention(e4m3): the pages are not aligned for vector loads");
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;
   Args a{q, (const unsigned char*)k, (const unsigned char*)v, (const unsigned char*)kv_scale, table, q_start, start_pos, out,
-         q_stride, out_stride, table_stride, table_width, 0, pages, nq, nkv, window, rows, scale * 1.4426950408889634f};
+         q_stride, out_stride, table_stride, table_width, 0, pages, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
+         nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   const long most_rows = (long)max_q_len * (nq / nkv);
-  const dim3 grid((unsigned)((most_rows + 15) / 16), nkv, reqs);
-  if (dtype == DT_BF16)
-    hipLaunchKernelGGL(attention_e4m3_kernel<bf16_t>, grid, dim3(64 * WAVES), 0, stream, a);
-  else
-    hipLaunchKernelGGL(attention_e4m3_kernel<float>, grid, dim3(64 * WAVES), 0, stream, a);
-  LLMLAB_LAUNCH_CHECK("attention(e4m3)");
-  return 0;
+  const int visible = window > 0 ? min(max_ctx_len, window + max_q_len) : max_ctx_len;
+  if (dtype == DT_F32)
+    return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
+  return most_rows > 16 && D <= 128 ? launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream)
+                                    : launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 }

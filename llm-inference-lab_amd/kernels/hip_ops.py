@@ -1114,7 +1114,8 @@ class HipOps:
                                    f"{lib.llmlab_attention_head_dim()}")
             lib.llmlab_paged_attention_e4m3.argtypes = [
                 _c_ptr, _c_int, _c_long, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int,
-                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_long, _c_int, _c_ptr]
+                _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_long, _c_int, _c_ptr, _c_size, _c_int,
+                _c_ptr]
             lib.llmlab_paged_attention_e4m3.restype = _c_int
             self._e4m3_attn[head_dim] = lib
             self.loaded_libraries.append(lib._name)
@@ -1202,6 +1203,8 @@ class HipOps:
         for t in (k_out, v_out):
             if tuple(t.shape) != (rows, num_kv_heads * head_dim):
                 raise ValueError(f"{what}: output {tuple(t.shape)} for {rows} rows of {num_kv_heads} heads of {head_dim}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{what}: outputs are not aligned to 16 bytes")
         self._rows_of(what, positions, row_req, rows)
         self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
         lib = self._mixer_lib("e4m3_cache")
@@ -1250,7 +1253,8 @@ class HipOps:
         args = [self._ptr(q), _dt(q), q_stride, num_heads, num_kv_heads, self._ptr(k_cache), self._ptr(v_cache),
                 self._ptr(kv_scale), k_cache.shape[0], self._ptr(block_table), block_table.stride(0), block_table.shape[1],
                 page_size, self._ptr(q_start), self._ptr(start_pos), 0, 0, 0, int(window) if window else 0, float(scale),
-                self._ptr(out), num_heads * head_dim, rows, None]
+                self._ptr(out), num_heads * head_dim, rows, self._ptr(self.workspace), self.workspace.numel(), self.num_cus,
+                None]
         return E4m3AttentionCall(self, lib, args,
                                  most_requests=min(q_start.numel() - 1, start_pos.numel(), block_table.shape[0]),
                                  most_context=block_table.shape[1] * page_size)
