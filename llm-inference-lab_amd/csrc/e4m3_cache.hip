@@ -106,6 +106,14 @@ __device__ __forceinline__ void store_numbers(T* dst, const float (&x)[N]) {
   }
 }
 
+// The four numbers of a word of codes (zeros where there is no page)
+__device__ __forceinline__ void decode_four(unsigned w, float size, bool there, float* x) {
+  x[0] = there ? __builtin_amdgcn_cvt_f32_fp8(w, 0) * size : 0.f;
+  x[1] = there ? __builtin_amdgcn_cvt_f32_fp8(w, 1) * size : 0.f;
+  x[2] = there ? __builtin_amdgcn_cvt_f32_fp8(w, 2) * size : 0.f;
+  x[3] = there ? __builtin_amdgcn_cvt_f32_fp8(w, 3) * size : 0.f;
+}
+
 // Four codes in a word, in their order
 __device__ __forceinline__ unsigned four_codes(const float (&x)[4], float inv) {
   return (unsigned)to_code(x[0], inv) | (unsigned)to_code(x[1], inv) << 8 | (unsigned)to_code(x[2], inv) << 16 |
@@ -276,53 +284,55 @@ __global__ __launch_bounds__(256) void read_kv_e4m3_kernel(T* k_out, T* v_out, i
       if (t >= n_rows) break;
       T* dst = k_out + (size_t)(r0 + t) * width + n * 16;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const unsigned w = codes[t][h];
-        const float x[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0) * size[t], __builtin_amdgcn_cvt_f32_fp8(w, 1) * size[t],
-                            __builtin_amdgcn_cvt_f32_fp8(w, 2) * size[t], __builtin_amdgcn_cvt_f32_fp8(w, 3) * size[t]};
-        float y[4];
+      for (int h = 0; h < 2; ++h) {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = page[t] >= 0 ? x[j] : 0.f;
-        store_numbers<T, 4, true>(dst + 4 * h, y);
+        for (int j = 0; j < 2; ++j) decode_four(codes[t][2 * h + j], size[t], page[t] >= 0, x + 4 * j);
+        store_numbers<T, 8, true>(dst + 8 * h, x);
       }
     }
   }
-  // values: 16 lanes a group of up to 64 numbers
-  for (int n = lane; n < a.nkv * groups * 16; n += 64) {
-    const int kvh = n / (groups * 16), m = n - kvh * groups * 16, group = m >> 4, c = m & 15;
+  // values: a lane has four neighbouring numbers of up to four 16-wide blocks, 64 consecutive bytes of the page
+  for (int n = lane; n < a.nkv * groups * 4; n += 64) {
+    const int kvh = n / (groups * 4), m = n - kvh * groups * 4, group = m >> 2, c = (m & 3) * 4;
     const int wide = min(4, sixteens - 4 * group);
-    unsigned codes[ROWS][4];
+    unsigned codes[ROWS][4][4];      // [row][number][block of the group]
+    float size[ROWS];
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
-      if (word && t > 0) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) codes[t][j] = codes[0][j];
-        continue;
-      }
       const size_t at = ((size_t)max(page[t], 0) * a.nkv + kvh) * a.page_size;
+      size[t] = a.pages > 0 ? power_of_byte(a.scale[2 * at + a.page_size + off[t]]) : 0.f;
       const unsigned* src = (const unsigned*)(a.v + at * d + (value_index(off[t], group * 64 + c, d) & ~(size_t)3));
-      if (a.pages <= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) codes[t][j] = 0;
-      } else if (wide == 4) {
-        const uint4v w = *(const uint4v*)src;
+      for (int i = 0; i < 4; ++i) {
+        if (word && t > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) codes[t][j] = w[j];
-      } else {
+          for (int j = 0; j < 4; ++j) codes[t][i][j] = codes[0][i][j];
+        } else if (a.pages <= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) codes[t][j] = src[min(j, wide - 1)];
+          for (int j = 0; j < 4; ++j) codes[t][i][j] = 0;
+        } else if (wide == 4) {
+          const uint4v w = *(const uint4v*)(src + 4 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) codes[t][i][j] = w[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) codes[t][i][j] = src[i * wide + min(j, wide - 1)];
+        }
       }
     }
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
       if (t >= n_rows) break;
-      const size_t at = ((size_t)max(page[t], 0) * a.nkv + kvh) * a.page_size;
-      const float size = page[t] >= 0 ? power_of_byte(a.scale[2 * at + a.page_size + off[t]]) : 0.f;
       T* dst = v_out + (size_t)(r0 + t) * width + (size_t)kvh * d + group * 64 + c;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < wide)
-          dst[j * 16] = from_float<T>(page[t] >= 0 ? __builtin_amdgcn_cvt_f32_fp8(codes[t][j] >> (8 * (off[t] & 3)), 0) * size : 0.f);
+      for (int j = 0; j < 4; ++j) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = page[t] >= 0 ? __builtin_amdgcn_cvt_f32_fp8(codes[t][i][j] >> (8 * (off[t] & 3)), 0) * size[t] : 0.f;
+        if (j < wide) store_numbers<T, 4, true>(dst + j * 16, x);
+      }
     }
   }
 }
@@ -382,7 +392,7 @@ extern "C" int llmlab_read_kv_e4m3(const void* k, const void* v, const void* sca
   const int rc = check_cache("read_kv_e4m3", a, rows);
   if (rc) return rc;
   if (rows == 0) return 0;
-  LLMLAB_REQUIRE((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 4 == 0, "read_kv_e4m3: the outputs are not aligned to 16 bytes");
+  LLMLAB_REQUIRE((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "read_kv_e4m3: the outputs are not aligned to 16 bytes");
   auto pick = [&](auto t) {
     typedef decltype(t) T;
     if (rows >= 4096)
