@@ -15,6 +15,7 @@
 //
 // float32 queries are taken as three bfloat16 parts (24 bits: nothing is lost), probabilities too, each part a
 // product of its own; the keys' and values' numbers are exact.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -391,6 +392,340 @@ __global__ __launch_bounds__(64 * NW) void attention_e4m3_split_kernel(Args a) {
   }
 }
 
+// ------------------------------------------------------------- many rows, codes staged in LDS
+// bfloat16 rows at heads of 64 and 128.  A block has RT tiles of 32 rows side by side, and P groups of waves that
+// take the staged keys in turn, 32 of every 32 P; the groups' sums meet in LDS at the end.  The codes come by direct loads
+// into LDS, in the cache's order, in two stages, one being multiplied while the other is on its way, one barrier a
+// stage, and become bfloat16 numbers behind the read from LDS: half the bytes there and on the way.  Products by
+// v_mfma_f32_32x32x16_bf16, transposed as above (lane l: row l % 32 of the tile, h = l / 32):
+//   S^T[key, row] = K . Q^T: element i of the 32 keys of a step is key 8 (i / 4) + 4 h + i % 4; a lane has the numbers
+//     16 (2 j + h) .. + 15 of its key, in two products, and the queries lie alike;
+//   O^T[d, row] = V^T . P^T: the keys of a block of 16 in the order {4 h .. + 3, 8 + 4 h .. + 3} for half h, which is what
+//     a lane holds of S^T; product i of a group of 64 numbers takes its 16-wide blocks i and 2 + i, as 8 bytes a lane
+//     hold blocks 0 and 1 (lanes 0 .. 15 of a half) or 2 and 3.
+// Every wave brings the scales of its group's keys itself, and makes float32 numbers of the values' ones in LDS.
+#define STAGED (HEAD_DIM == 64 || HEAD_DIM == 128)
+#if STAGED
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
+
+// 16 bytes (a word) a lane from the cache to consecutive memory of LDS.  One statement with the m0 that the load reads:
+// between two the compiler may use m0 itself.  The compiler does not see into the statements, so the five wait
+// states that a load needs behind a vector instruction which wrote its scalar address (a v_readlane that brings back a
+// spilled pointer, say) are in them.
+__device__ __forceinline__ void load_1k(unsigned lane_offset, const unsigned char* base, unsigned to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void load_words(unsigned lane_offset, const unsigned char* base, unsigned to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" : : "v"(lane_offset), "s"(base), "s"(to) : "memory", "m0");
+}
+// A number of the block table, waited for on the spot (the compiler, which does not see it, would wait for all loads on
+// their way wherever a branch with a load of its own ends)
+__device__ __forceinline__ int table_entry(const int* table, int at) {
+  int v;
+  asm volatile("s_nop 4\n\tglobal_load_dword %0, %1, %2\n\ts_waitcnt vmcnt(0)" : "=&v"(v) : "v"(at * 4), "s"(table) : "memory");
+  return v;
+}
+
+template <int RT, int P>
+struct StagedSizes {
+  static constexpr int NW = RT * P, KT = 32 * P;
+  static constexpr int V_AT = KT * D, SCALES_AT = 2 * KT * D, STAGE = SCALES_AT + NW * 512;
+  static constexpr int STAGES = 2 * STAGE, SUMS = RT * (P - 1) * 32 * D * 4;
+  static constexpr int LDS = (STAGES > SUMS ? STAGES : SUMS) + NW * 32 * 4 * 3;
+};
+
+template <int RT, int P>
+__global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
+  typedef StagedSizes<RT, P> Z;
+  constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DV = D / 32;
+  constexpr int PIECES = KT * D / 1024;                          // loads of 1 KB of a stage's keys, and of its values
+  constexpr int EACH = PIECES * 2 / NW;                          // ... of a wave
+  constexpr int HALF = EACH > 1 ? EACH / 2 : 1;                  // ... of keys, and of values (one: keys by even waves)
+  constexpr int PB = D / 64;                                     // pieces of a block of 16 keys
+  constexpr int BLOCKS = HALF > PB ? HALF / PB : 1;              // blocks of 16 that a wave's pieces belong to
+  static_assert(EACH * NW == PIECES * 2 && (EACH == 1 || EACH % 2 == 0), "whole loads a wave");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Z::LDS];
+  float* const own = (float*)(lds + (Z::STAGES > Z::SUMS ? Z::STAGES : Z::SUMS));
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rt = wave % RT, ph = wave / RT, col = lane & 31, h = lane >> 5, odd = (lane >> 4) & 1, c = lane & 15;
+  const int G = a.nq / a.nkv;
+  // the tiles with the longest histories of all kv heads and requests first (or along y and z)
+  int b = blockIdx.z, kvh = blockIdx.y, rank = blockIdx.x;
+  if (gridDim.y == 1 && gridDim.z == 1) {
+    const int per = a.nkv * a.reqs, at = rank % per;
+    rank /= per;
+    kvh = at % a.nkv;
+    b = at / a.nkv;
+  }
+  const int r0 = a.q_start[b], count = a.q_start[b + 1] - r0, before = a.start_pos[b];
+  const int total = count * G, block_row0 = (tiles - 1 - rank) * RT * 32;
+  if (block_row0 >= total || r0 < 0 || count > a.rows - r0) return;
+  const int row0 = block_row0 + rt * 32, row = row0 + col;
+  const bool valid = row < total;
+  const int tok = valid ? row / G : 0, head = kvh * G + (valid ? row - tok * G : 0);
+  // (a key is seen if it is no further than pos - lo behind lo: one comparison; a row that sees none has its lo behind all keys)
+  const int pos = valid ? before + tok : -1, lo = pos < 0 ? 1 << 30 : a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  const int lane_key = 4 * h - lo;
+  const unsigned span = pos < 0 ? 0 : pos - lo;
+  // the keys that the block's rows see; up to p_first and from full_lo on every row of the wave sees them
+  const int last = min(row0 + 32, total) - 1, block_last = min(block_row0 + RT * 32, total) - 1;
+  const int p_first = before + row0 / G, p_last = row0 < total ? before + last / G : -1;
+  const int full_lo = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
+  const int key_hi = max(before + block_last / G, 0);
+  const int key_lo = a.window > 0 ? max(0, before + block_row0 / G - a.window + 1) : 0;
+  const int tile_lo = key_lo / KT, tile_hi = key_hi / KT;
+  const int block_lo = key_lo & ~15, block_hi = key_hi & ~15;
+
+  // Of 64 tiles at a time, tile base + l in lane l: where the blocks of 16 keys are that the wave brings, counted in such
+  // blocks, and where the scales of its group's two, counted in 16 bytes; negative: not there, read as page 0 and seen
+  // by nobody.  Blocks that no row sees read one that some row does.
+  const int* const table = a.table + (size_t)b * a.table_stride;
+  const int shift = a.page_shift, page_blocks = 1 << (shift - 4);
+  const int piece0 = EACH > 1 ? wave * HALF : wave >> 1;
+  constexpr unsigned HERE = 0x7fffffffu;
+  unsigned where[BLOCKS], scales_where[2];
+  int base = tile_lo;
+  auto locate = [&](int from) {
+    base = from;
+    auto block_at = [&](int block16, bool of_scales) {
+      const int key = max(min(min(from + lane, tile_hi) * KT + block16 * 16, block_hi), block_lo), at = key >> shift;
+      int page = -1;
+      if (a.table_width > 0) page = table_entry(table, min(at, a.table_width - 1));
+      const bool there = at < a.table_width && page >= 0 && page < a.pages;
+      const unsigned row = (unsigned)(there ? page : 0) * a.nkv + kvh;
+      return (row * (of_scales ? 2 : 1) * page_blocks + ((key >> 4) & (page_blocks - 1))) | (there ? 0u : ~HERE);
+    };
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n) where[n] = block_at(piece0 / PB + n, false);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) scales_where[n] = block_at(ph * 2 + n, true);
+  };
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  const unsigned scales_from = (lane & 3) * 4 + (lane >> 2 & 1) * page_blocks * 16;      // a word of the keys' or the values' scales
+  // (the result: which blocks of the wave's group are there)
+  auto fetch = [&](int tile, int slot) {
+    if (tile - base >= 64) locate(tile);
+    const unsigned to = lds0 + slot * Z::STAGE;
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n) {
+      const unsigned block = (unsigned)__builtin_amdgcn_readlane((int)where[n], tile - base) & HERE;
+      const size_t at = (size_t)block * (16 * D) + piece0 % PB * 1024;
+#pragma unroll
+      for (int i = 0; i < HALF / BLOCKS; ++i) {
+        const unsigned to_piece = to + (piece0 + n * PB + i) * 1024;
+        if constexpr (EACH > 1) {
+          load_1k(lane * 16, a.k + at + i * 1024, to_piece);
+          load_1k(lane * 16, a.v + at + i * 1024, to_piece + Z::V_AT);
+        } else {
+          load_1k(lane * 16, (wave & 1 ? a.v : a.k) + at, wave & 1 ? to_piece + Z::V_AT : to_piece);
+        }
+      }
+    }
+    unsigned there = 0;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const unsigned at = (unsigned)__builtin_amdgcn_readlane((int)scales_where[n], tile - base);
+      there |= at <= HERE ? 1u << n : 0u;
+      load_words(scales_from, a.scale + (size_t)(at & HERE) * 16, to + Z::SCALES_AT + wave * 512 + n * 256);
+    }
+    return there;
+  };
+
+  bf16x8 q[DK];
+  {
+    const bf16_t* qp = (const bf16_t*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
+#pragma unroll
+    for (int k = 0; k < DK; ++k) q[k] = *(const bf16x8*)(qp + ((k >> 1) * 2 + h) * 16 + (k & 1) * 8);
+  }
+  locate(tile_lo);
+  // (waited for here, with the table: in the loop it would be waited for, with all that is on its way, in every step)
+#pragma unroll
+  for (int k = 0; k < DK; ++k) {
+    const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    q[k] = valid ? q[k] : zero;
+    asm volatile("" : "+v"(q[k]));
+  }
+  floatx16 o[DV];
+#pragma unroll
+  for (int i = 0; i < DV; ++i)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
+  float m = NEG_INF, l = 0.f;
+  unsigned there_next = fetch(tile_lo, 0);
+  float* const own_scales = own + wave * 32;
+  const int k_at = (ph * 2 + odd) * 16 * D + h * 256 + c * 16, v_at = Z::V_AT + ph * 32 * D + h * 256 + c * 16 + odd * 8;
+  for (int tile = tile_lo; tile <= tile_hi; ++tile) {
+    // this tile's loads are in (the wave's own; behind the barrier, all), and the tile before is read by all
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    const int slot = (tile - tile_lo) & 1;
+    const unsigned char* const stage = lds + slot * Z::STAGE;
+    const unsigned char* const scales = stage + Z::SCALES_AT + wave * 512 + odd * 256 + c;
+    uint4v kc[DK / 2];
+#pragma unroll
+    for (int j = 0; j < DK / 2; ++j) kc[j] = *(const uint4v*)(stage + k_at + j * 512);
+    const float ks = power_of_byte(scales[0]);
+    const float own_scale = power_of_byte(min((unsigned)scales[16], 254u));      // (finite: times a probability of zero it is zero)
+    if (h == 0) own_scales[col] = own_scale;
+    const unsigned there = there_next;
+    there_next = fetch(tile + 1, slot ^ 1);
+    const int kb0 = tile * KT + ph * 32;
+    floatx16 s;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) s[x] = 0.f;
+#pragma unroll
+    for (int j = 0; j < DK / 2; ++j) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][0], kc[j][1], ks), q[2 * j], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][2], kc[j][3], ks), q[2 * j + 1], s, 0, 0, 0);
+    }
+    // the values' codes travel while the maximum is found: [block of 16][group of 64][quad h or 2 + h], two blocks of 16 of d each
+    typedef unsigned uint2v __attribute__((ext_vector_type(2)));
+    uint2v vc[2][D / 64][2];
+#pragma unroll
+    for (int block = 0; block < 2; ++block)
+#pragma unroll
+      for (int group = 0; group < D / 64; ++group)
+#pragma unroll
+        for (int two = 0; two < 2; ++two) vc[block][group][two] = *(const uint2v*)(stage + v_at + block * 16 * D + group * 1024 + two * 512);
+    const bool masked = !(kb0 + 31 <= p_first && kb0 >= full_lo && there == 3);
+    auto sees = [&](int i) {
+      return (there >> (i >> 3) & 1) != 0 && (unsigned)(kb0 + 8 * (i >> 2) + (i & 3) + lane_key) <= span;
+    };
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : NEG_INF;
+      // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not keep
+      // out of the product: they become zeros, and the rows that do see them become no numbers.
+      bool strange = false;
+#pragma unroll
+      for (int block = 0; block < 2; ++block)
+#pragma unroll
+        for (int group = 0; group < D / 64; ++group)
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            strange |= (((vc[block][group][n >> 1][n & 1] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+      if (__any(strange)) {
+#pragma unroll
+        for (int block = 0; block < 2; ++block) {
+          bf16x8 seen;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) seen[i] = sees(block * 8 + i) ? (bf16_t)1.f : (bf16_t)0.f;
+#pragma unroll
+          for (int group = 0; group < D / 64; ++group)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              bf16x8 bad;
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const bool nan = ((vc[block][group][x >> 2][i] >> (8 * (x & 3))) & 0x7fu) == 0x7fu;
+                bad[x] = nan ? (bf16_t)1.f : (bf16_t)0.f;
+                if (nan) vc[block][group][x >> 2][i] &= ~(0xffu << (8 * (x & 3)));
+              }
+              floatx16 hits;
+#pragma unroll
+              for (int x = 0; x < 16; ++x) hits[x] = 0.f;
+              hits = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bad, seen, hits, 0, 0, 0);
+#pragma unroll
+              for (int x = 0; x < 16; ++x)
+                if (hits[x] > 0.f) o[group * 2 + i][x] = __builtin_nanf("");
+            }
+        }
+      }
+    }
+    float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+    for (int x = 0; x < 16; x += 2) mx[(x >> 1) & 3] = fmaxf(fmaxf(s[x], s[x + 1]), mx[(x >> 1) & 3]);
+    mx[0] = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), mx[2]), mx[3]);
+    if (__any(mx[0] * a.scale2 > m + LAZY_MAX)) {      // some row's maximum grew: rescale what is summed so far
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx[0]), __float_as_uint(mx[0]), false, false);
+      mx[0] = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * a.scale2;
+      const bool grow = mx[0] > m + LAZY_MAX;
+      const float m_new = grow ? mx[0] : m, alpha = grow ? fast_exp2(m - m_new) : 1.f;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DV; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+      m = m_new;
+    }
+    const float neg_m = m == NEG_INF ? 0.f : -m;      // (no key seen yet: every p is 2^-inf = 0)
+#pragma unroll
+    for (int block = 0; block < 2; ++block) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = fast_exp2(fmaf(s[block * 8 + i], a.scale2, neg_m));
+      l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      const floatx4 w0 = *(const floatx4*)(own_scales + block * 16 + 4 * h), w1 = *(const floatx4*)(own_scales + block * 16 + 8 + 4 * h);
+      bf16x8 pf;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pf[i] = (bf16_t)(p[i] * (i < 4 ? w0[i & 3] : w1[i & 3]));
+#pragma unroll
+      for (int group = 0; group < D / 64; ++group)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(vc[block][group][0][i], vc[block][group][1][i], 1.f), pf,
+                                                                     o[group * 2 + i], 0, 0, 0);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);      // the last loads (of a tile past the end) are in, and the stages read
+  __syncthreads();
+  l += __shfl_xor(l, 32, WAVE);
+
+  // piece n of a row, four numbers: registers 4 (n % 4) .. + 3 of sum n / 4
+  auto place = [&](int n) { return (n >> 3) * 64 + (((n & 3) >> 1) * 2 + ((n >> 2) & 1)) * 16 + (n & 1) * 8 + h * 4; };
+  auto piece = [&](int n) { return floatx4{o[n >> 2][4 * (n & 3)], o[n >> 2][4 * (n & 3) + 1], o[n >> 2][4 * (n & 3) + 2], o[n >> 2][4 * (n & 3) + 3]}; };
+  if constexpr (P == 1) {
+    if (valid)
+#pragma unroll
+      for (int n = 0; n < DV * 4; ++n) write_output<bf16_t>(a, r0 + tok, head, place(n), piece(n), l);
+  } else {
+    // group ph puts the pieces ph, ph + P, .. of its rows together; the others' it finds in LDS
+    constexpr int SHARES = DV * 4 / P;
+    static_assert(SHARES * P == DV * 4, "whole shares");
+    floatx4* const left = (floatx4*)lds;      // [wave][share][group but the wave's own][lane]
+    float* const s_m = own + NW * 32;
+    float* const s_l = s_m + NW * 32;
+    if (h == 0) {
+      s_m[wave * 32 + col] = m;
+      s_l[wave * 32 + col] = l;
+    }
+    floatx4 mine[SHARES];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int n = 0; n < SHARES; ++n) {
+        if (p == ph) mine[n] = piece(n * P + p);
+        else left[((wave * SHARES + n) * (P - 1) + (p > ph ? p - 1 : p)) * 64 + lane] = piece(n * P + p);
+      }
+    __syncthreads();
+    float w[P], top = NEG_INF, weight = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      w[p] = s_m[(p * RT + rt) * 32 + col];
+      top = fmaxf(top, w[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      // (no maximum: no key that the row sees, sums of zero, or scores that are no numbers, and sums likewise)
+      w[p] = w[p] == NEG_INF ? 1.f : fast_exp2(w[p] - top);
+      weight += w[p] * s_l[(p * RT + rt) * 32 + col];
+    }
+#pragma unroll
+    for (int n = 0; n < SHARES; ++n) {
+      floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        v += w[p] * (p == ph ? mine[n] : left[(((p * RT + rt) * SHARES + n) * (P - 1) + (ph > p ? ph - 1 : ph)) * 64 + lane]);
+      if (valid) write_output<bf16_t>(a, r0 + tok, head, place(n * P + ph), v, weight);
+    }
+  }
+}
+#endif  // STAGED
+
 // The splits of a row put together: a wave a (row, head), four numbers a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
@@ -428,43 +763,72 @@ __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
 extern "C" int llmlab_attention_head_dim() { return D; }
 
-// For measurements and tests: the number of key splits (0: by the rule)
-static int g_force_splits = 0, g_force_waves = 0;
-extern "C" void llmlab_debug_attention_e4m3(int splits, int waves) {
+// For measurements and tests: the number of key splits (0: by the rule) and the form of the launch (0: by the rule, else one
+// of those below where it exists)
+static int g_force_splits = 0, g_force_form = 0;
+extern "C" void llmlab_debug_attention_e4m3(int splits, int form) {
   g_force_splits = splits;
-  g_force_waves = waves;
+  g_force_form = form;
 }
 
-// Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys
-// for each of its waves.
+constexpr int SPLIT_WAVES = 4;
+// Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys.
 static int key_splits(long blocks, int visible, int num_cus) {
   if (blocks >= num_cus) return 1;
   const long steps = (visible + 31) / 32, most = (steps + 7) / 8;
-  return (int)max(1L, min(min(2L * num_cus / blocks, most), 128L));
+  return (int)std::max(1L, std::min(std::min(2L * num_cus / blocks, most), 128L));
 }
 
-template <typename T, int QB, int NW>
-static void launch_split_waves(const Args& a, dim3 grid, hipStream_t stream) {
-  hipLaunchKernelGGL((attention_e4m3_split_kernel<T, QB, NW>), grid, dim3(64 * NW), 0, stream, a);
+// The form of a bfloat16 launch at heads of 64 and 128: the one whose time is the least by an estimate, rounds of blocks (`more`
+// for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
+// its steps of 32 keys x a step), in us as fitted to 1,150 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
+// behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
+// the picks lose 0.7 % (heads of 64) and 1 % (128) to the best of all, 20 % at worst (200 others: 1.3 %, 15 %).  Up to 16 rows a tile's keys are
+// split over waves and blocks; of more rows so, too, where they are few and the keys many.
+// us, split / 2x4 / 2x2 / 4x1, heads of 128: 25 rows of 456 (request, kv head) pairs and 182 keys
+// 17.9 / 18.0 / 12.0 / 15.2; 336 rows of 24 behind 3,300 67 / 38 / 48 / 86; 36 of 4 behind 3,000 13 / 33 / 44 / 77; 3,216 of 4
+// and 536 20 / 14.5 / 14.2 / 21; 12,296 of 6 behind 768 134 / 84 / 63 / 59; 2,176 of 120 and 317 270 / 152 / 85 / 74.
+enum { FORM_SPLIT = 1, FORM_2x4, FORM_2x2, FORM_4x1 };
+#if STAGED
+static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
+  if (most_rows <= 16) return FORM_SPLIT;
+  struct Form { int rows, groups; float blocks_a_unit, start, step, more, least; };
+  constexpr Form forms[] = {{32, SPLIT_WAVES, 2.f, D == 64 ? 4.95f : 9.5f, D == 64 ? 1.05f : 2.1f, D == 64 ? .66f : .57f, D == 64 ? 1.f : .7f},
+                            {64, 4, 1.f, D == 64 ? 5.3f : 7.8f, D == 64 ? .9f : 1.27f, .5f, D == 64 ? 1.1f : 1.f},
+                            {64, 2, D == 64 ? 3.f : 2.f, D == 64 ? 5.8f : 7.9f, .9f, D == 64 ? .58f : .65f, D == 64 ? .93f : .84f},
+                            {128, 1, D == 64 ? 3.f : 2.f, D == 64 ? 6.9f : 9.2f, D == 64 ? .72f : .79f, .74f, .9f}};
+  constexpr float MERGE = D == 64 ? 2.7f : 1.9f;
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const Form& f = forms[i];
+    const long tiles = (most_rows + f.rows - 1) / f.rows * pairs;
+    const int splits = i == 0 ? key_splits(tiles, visible, num_cus) : 1;
+    const float steps = splits > 1 ? (float)visible / (32 * f.groups * splits) : (float)walk / (32 * f.groups);
+    const float rounds = (float)tiles * splits / (f.blocks_a_unit * num_cus) + f.more;
+    const float time = std::max(rounds, f.least) * (f.start + std::max(steps, 1.f) * f.step) + (splits > 1 ? MERGE : 0.f);
+    if (i == 0 || time < least) {
+      least = time;
+      best = i + 1;
+    }
+  }
+  return best;
 }
+#endif
 
 template <typename T, int QB>
 static int launch_split(Args a, long most_rows, int visible, float* workspace, size_t workspace_floats, int num_cus,
                         hipStream_t stream) {
   const long tiles = (most_rows + 16 * QB - 1) / (16 * QB);
-  a.splits = g_force_splits > 0 ? g_force_splits : key_splits(tiles * a.nkv * a.reqs, visible, num_cus > 0 ? num_cus : 256);
+  a.splits = g_force_splits > 0 ? g_force_splits : key_splits(tiles * a.nkv * a.reqs, visible, num_cus);
   const size_t each = (size_t)a.rows * a.nq * (D + 2);
-  a.splits = (int)max((size_t)1, min((size_t)min(a.splits, 65535 / a.nkv), workspace_floats / max(each, (size_t)1)));
+  a.splits = (int)std::max((size_t)1, std::min((size_t)std::min(a.splits, 65535 / a.nkv), workspace_floats / std::max(each, (size_t)1)));
   if (a.splits > 1) {
     a.o_part = workspace;
     a.ml_part = workspace + (size_t)a.rows * a.nq * a.splits * D;
   }
-  const dim3 grid((unsigned)tiles, a.nkv * a.splits, a.reqs);
-  constexpr int WIDE = split_lds_floats<QB, 8>() * 4 <= 80 * 1024 ? 8 : 4;
-  if (g_force_waves == 8)
-    launch_split_waves<T, QB, WIDE>(a, grid, stream);
-  else
-    launch_split_waves<T, QB, 4>(a, grid, stream);
+  hipLaunchKernelGGL((attention_e4m3_split_kernel<T, QB, SPLIT_WAVES>), dim3((unsigned)tiles, a.nkv * a.splits, a.reqs),
+                     dim3(64 * SPLIT_WAVES), 0, stream, a);
   LLMLAB_LAUNCH_CHECK("attention(e4m3)");
   if (a.splits > 1) {
     hipLaunchKernelGGL(attention_e4m3_merge_kernel<T>, dim3((unsigned)(((long)a.rows * a.nq + 3) / 4)), dim3(256), 0, stream, a);
@@ -472,6 +836,17 @@ static int launch_split(Args a, long most_rows, int visible, float* workspace, s
   }
   return 0;
 }
+
+#if STAGED
+template <int RT, int P>
+static int launch_staged(const Args& a, long most_rows, hipStream_t stream) {
+  const long tiles = (most_rows + 32 * RT - 1) / (32 * RT), blocks = tiles * a.nkv * a.reqs;
+  const dim3 grid = blocks * 64 * RT * P <= 0xffffffffL ? dim3((unsigned)blocks) : dim3((unsigned)tiles, a.nkv, a.reqs);
+  hipLaunchKernelGGL((attention_e4m3_staged_kernel<RT, P>), grid, dim3(64 * RT * P), 0, stream, a, (int)tiles);
+  LLMLAB_LAUNCH_CHECK("attention(e4m3, staged)");
+  return 0;
+}
+#endif
 
 extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stride, int nq, int nkv, const void* k, const void* v,
                                            const void* kv_scale, int pages, const int* table, int table_stride, int table_width,
@@ -493,9 +868,17 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
          nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   const long most_rows = (long)max_q_len * (nq / nkv);
-  const int visible = window > 0 ? min(max_ctx_len, window + max_q_len) : max_ctx_len;
+  const int visible = window > 0 ? (int)std::min((long)max_ctx_len, (long)window + max_q_len) : max_ctx_len;
+  if (num_cus <= 0) num_cus = 256;
   if (dtype == DT_F32)
     return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
+#if STAGED
+  const int middle = max_ctx_len - max_q_len / 2, walk = window > 0 ? std::min(window, middle) : middle;
+  const int form = g_force_form > 0 ? g_force_form : launch_form(most_rows, (long)nkv * reqs, walk, visible, num_cus);
+  if (form == FORM_2x4) return launch_staged<2, 4>(a, most_rows, stream);
+  if (form == FORM_2x2) return launch_staged<2, 2>(a, most_rows, stream);
+  if (form == FORM_4x1) return launch_staged<4, 1>(a, most_rows, stream);
+#endif
   return most_rows > 16 && D <= 128 ? launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream)
                                     : launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 }

@@ -128,7 +128,7 @@ class KernelDebug:
               attention_merge_kernel: Optional[int] = None,
               attention_merge_in_place: Optional[int] = None, attention_two_launches: Optional[int] = None,
               attention_one_launch: Optional[int] = None, attention_small_tiles: Optional[int] = None,
-              f32_fma: Optional[bool] = None, **rules):
+              e4m3_attention: Optional[Tuple[int, int, int]] = None, f32_fma: Optional[bool] = None, **rules):
         """``gemm_tile``: 64 (64 x 64), 130 (64 x 128), 129 (128 x 128), 131 (128 x 256), 132 (256 x
         256), 133 (192 x 256), 134 / 135 / 136 (64 x 96 / 160 / 224), 137 (128 x 160) or 138 / 139 / 140 (128 x 128, 128 x 192,
         192 x 128 by direct loads, eight waves); -131: the choice among the first three; -256 and below: the
@@ -147,6 +147,9 @@ class KernelDebug:
         a head size; a mixed step's decoding requests and its portions get a launch each also
         where one launch would serve both, or one launch wherever there is a kernel for both; ``attention_small_tiles``:
         a head size (up to 128); one launch with the portions by tiles of 16 rows.
+        ``e4m3_attention``: (head size, key splits, form) of attention over 8-bit keys and values: 0 splits as the kernel
+        chooses; form 0 as it chooses, 1 = the waves of a block split the keys of a tile, and at heads of 64 and 128 in bfloat16
+        2 to 4 = keys staged in LDS, blocks of 2 tiles of 32 rows by 4 groups of waves, 2 by 2, 4 by 1.
         ``f32_fma``: float32 products of many rows by the plain FMA kernel instead of the
         matrix cores.  Other keywords: fields of ``DispatchRules`` for the time of the block."""
         ops = self._ops
@@ -156,7 +159,7 @@ class KernelDebug:
             if not hasattr(ops.rules, key):
                 raise TypeError(f"no dispatch rule named '{key}'")
             setattr(ops.rules, key, value)
-        lib = plib = mlib = tlib = None
+        lib = plib = mlib = tlib = elib = None
         ops.debug_epoch += 1
         try:
             if attention_merge_kernel is not None:
@@ -188,6 +191,9 @@ class KernelDebug:
             if attention_splits is not None:
                 lib = ops._attention_lib(int(attention_splits[0]))
                 lib.llmlab_debug_attention_splits(int(attention_splits[1]))
+            if e4m3_attention is not None:
+                elib = ops._e4m3_attention_lib(int(e4m3_attention[0]))
+                elib.llmlab_debug_attention_e4m3(int(e4m3_attention[1]), int(e4m3_attention[2]))
             yield ops
         finally:
             ops.debug_epoch += 1
@@ -208,3 +214,5 @@ class KernelDebug:
                 mlib.llmlab_debug_attention_merge_kernel(0)
             if tlib is not None:
                 tlib.llmlab_debug_attention_two_launches(0)
+            if elib is not None:
+                elib.llmlab_debug_attention_e4m3(0, 0)

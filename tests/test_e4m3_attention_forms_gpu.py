@@ -1,0 +1,89 @@
+"""Every form of the launch of attention over 8-bit keys and values, whichever the sizes would pick: the tests of
+test_e4m3_attention_gpu.py with the form forced, and sizes at which a form can go wrong."""
+import math
+
+import pytest
+import torch
+
+import plain_e4m3 as plain
+import test_e4m3_attention_gpu as whole
+from e4m3_cases import Cache, ragged
+from test_e4m3_attention_gpu import check, ops, queries, run  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+FORMS = [1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq,nkv,page,lengths,counts,window", [
+    (1, 1, 16, [1], [1], None),                                    # one row, one key
+    (14, 2, 64, [700], [1], None),
+    (4, 2, 64, [1, 64, 65, 127, 300], [1, 1, 1, 1, 1], None),
+    (28, 4, 64, [500, 33, 5, 256], [5, 5, 5, 5], None),
+    (12, 2, 64, [300, 300], [1, 50], 64),
+    (4, 4, 64, [400], [3], 1),
+    (16, 2, 16, [700, 300], [61, 50], 200),
+    (2, 2, 64, [333], [200], None),
+    (14, 2, 64, [290, 40], [290, 33], None),                        # from a prompt's start, ragged
+    (2, 1, 16, [16 * 300 + 5], [37], None),                         # more tiles than a wave looks up pages for at a time
+    (2, 1, 16, [4700], [70], 900),
+    (1, 1, 256, [513], [129], None),                                # a row past a tile of 128
+])
+def test_forms(ops, form, d, nq, nkv, page, lengths, counts, window):      # noqa: F811
+    with ops.debug.force(e4m3_attention=(d, 0, form)):
+        check(ops, nq, nkv, d, page, lengths, counts, "bf16", window, seed=form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_what_stays_with_its_rows(ops, form):      # noqa: F811
+    with ops.debug.force(e4m3_attention=(64, 0, form)):
+        whole.test_pages_that_are_not_there(ops)
+        for counts in ([4], [70]):
+            whole.test_what_is_not_a_number_stays_with_the_rows_that_see_it(ops, "bf16", counts)
+        whole.test_requests_without_tokens_and_rows_behind_the_last(ops)
+        whole.test_large_scores(ops)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_missing_pages_in_bfloat16(ops, form, d):      # noqa: F811
+    """Whole tiles of keys without a page, the first, the last and some between; a request without any."""
+    nq, nkv, page = 4, 2, 16
+    lengths, counts = [700, 40, 300], [40, 40, 3]
+    cache = Cache(lengths, nkv, d, page).fill()
+    for slot in [0, 1, 2, 3, 4, 5, 6, 7, 8, 20, 33, 43]:
+        cache.table[0, slot] = -1
+    cache.table[0, 21] = cache.pages
+    cache.table[1] = -1
+    q_start, start_pos, positions, _ = ragged(lengths, counts)
+    q = queries(len(positions), nq, d, "bf16", 1)
+    with ops.debug.force(e4m3_attention=(d, 0, form)):
+        got = run(ops, cache, q, nq, q_start, start_pos, lengths, counts, None, 0.002).double().view(-1, nq, d)
+    want, spread, reach = plain.attention(q, nq, nkv, d, cache.k, cache.v, cache.scale, cache.table, page, q_start, start_pos, 3,
+                                          None, 0.002)
+    assert bool(((got - want).abs() <= plain.tolerance(torch.bfloat16, want, spread, reach, 700, d)).all())
+    assert not bool(got[40:80].any())
+
+
+@pytest.mark.parametrize("splits", [1, 2, 7, 64])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_key_splits(ops, splits, dtype):      # noqa: F811
+    """Splits that leave some blocks without a key."""
+    with ops.debug.force(e4m3_attention=(64, splits, 1)):
+        check(ops, 14, 2, 64, 64, [700, 3, 90], [1, 1, 2], dtype)
+        check(ops, 4, 2, 64, 16, [700, 30], [20, 11], dtype, window=100)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_the_same_every_time(ops, form):      # noqa: F811
+    """Sums are taken in one order: the same bits from every run."""
+    nq, nkv, d, page = 28, 4, 128, 64
+    lengths, counts = [1500, 700, 1100], [90, 200, 1]
+    cache = Cache(lengths, nkv, d, page).fill()
+    q_start, start_pos, positions, _ = ragged(lengths, counts)
+    q = queries(len(positions), nq, d, "bf16", 1)
+    dev = cache.on(whole.DEVICE)
+    with ops.debug.force(e4m3_attention=(d, 0, form)):
+        outs = [run(ops, cache, q, nq, q_start, start_pos, lengths, counts, None, 1 / math.sqrt(d) / 64, dev=dev) for _ in range(4)]
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
