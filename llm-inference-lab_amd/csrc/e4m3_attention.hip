@@ -107,8 +107,8 @@ struct Step {
 // The rows of one tile as a lane has them (row 16 qb + lane % 16), and what is summed for them so far.
 template <int QB, int PARTS>
 struct Rows {
-  bool valid[QB];
-  int pos[QB], lo[QB];
+  int lo[QB];            // the first key that the row sees (a row past the last, or in front of all keys: behind all keys)
+  unsigned span[QB];     // and how many follow it
   bf16x8 q[QB][PARTS][KP][2];
   floatx4 o[QB][DB];
   float m[QB], l[QB];
@@ -121,17 +121,17 @@ __device__ __forceinline__ void load_rows(const Args& a, Rows<QB, PARTS>& r, int
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int row = row0 + qb * 16 + c;
-    r.valid[qb] = row < total;
-    const int tok = r.valid[qb] ? row / G : 0, head = kvh * G + (r.valid[qb] ? row - tok * G : 0);
-    r.pos[qb] = before + tok;
-    r.lo[qb] = a.window > 0 ? max(0, r.pos[qb] - a.window + 1) : 0;
+    const bool valid = row < total;
+    const int tok = valid ? row / G : 0, head = kvh * G + (valid ? row - tok * G : 0), pos = valid ? before + tok : -1;
+    r.lo[qb] = pos < 0 ? 1 << 30 : a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    r.span[qb] = pos < 0 ? 0 : pos - r.lo[qb];
     const T* q = (const T*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int dd = kp * 64 + g * 16 + h * 8;
-        const bool in = r.valid[qb] && dd < D;      // (D is a multiple of 16: eight numbers are in or out together)
+        const bool in = valid && dd < D;      // (D is a multiple of 16: eight numbers are in or out together)
         if constexpr (PARTS == 1) {
           const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
           const bf16x8 x = *(const bf16x8*)(q + (in ? dd : 0));
@@ -180,22 +180,25 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
   }
   float vs[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = power_of_byte((f.vs[i >> 2] >> (8 * (i & 3))) & 255u);
+  for (int i = 0; i < 8; ++i) {
+    const unsigned byte = (f.vs[i >> 2] >> (8 * (i & 3))) & 255u;
+    vs[i] = power_of_byte(MASKED ? min(byte, 254u) : byte);      // (finite where it may be any byte: times a probability of zero it is zero)
+  }
   auto key = [&](int i) { return kb + (i >> 2) * 16 + g * 4 + (i & 3); };
-  auto sees = [&](int qb, int i) { return f.there[i >> 2] && r.valid[qb] && key(i) <= r.pos[qb] && key(i) >= r.lo[qb]; };
+  auto sees = [&](int qb, int i) { return f.there[i >> 2] && (unsigned)(key(i) - r.lo[qb]) <= r.span[qb]; };
   bf16x8 pf[QB][PARTS];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = s[i >> 2][qb][i & 3] * a.scale2;
+      p[i] = s[i >> 2][qb][i & 3];
       if (MASKED && !sees(qb, i)) p[i] = NEG_INF;
     }
-    float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-    mx = max_across_rows(mx);
-    const bool grow = mx > r.m[qb] + LAZY_MAX;
-    if (__any(grow)) {
+    float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), p[2]), fmaxf(fmaxf(p[3], p[4]), fmaxf(fmaxf(p[5], p[6]), p[7])));
+    if (__any(mx * a.scale2 > r.m[qb] + LAZY_MAX)) {      // some row's maximum grew: rescale what is summed so far
+      mx = max_across_rows(mx) * a.scale2;
+      const bool grow = mx > r.m[qb] + LAZY_MAX;
       const float m_new = grow ? mx : r.m[qb], alpha = grow ? fast_exp2(r.m[qb] - m_new) : 1.f;
       r.l[qb] *= alpha;
 #pragma unroll
@@ -204,13 +207,12 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
     }
     const float neg_m = MASKED && r.m[qb] == NEG_INF ? 0.f : -r.m[qb];      // (no key seen yet: every p is 2^-inf = 0)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(p[i] + neg_m);
+    for (int i = 0; i < 8; ++i) p[i] = fast_exp2(fmaf(p[i], a.scale2, neg_m));
     r.l[qb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float w = MASKED && !sees(qb, i) ? 0.f : p[i] * vs[i];      // (the scale of a place not seen is not used)
       bf16_t part[PARTS];
-      split<PARTS>(w, part);
+      split<PARTS>(p[i] * vs[i], part);
 #pragma unroll
       for (int n = 0; n < PARTS; ++n) pf[qb][n][i] = part[n];
     }
@@ -266,7 +268,7 @@ template <int QB, int NW>
 constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
 
 template <typename T, int QB, int NW>
-__global__ __launch_bounds__(64 * NW) void attention_e4m3_split_kernel(Args a) {
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attention_e4m3_split_kernel(Args a) {
   constexpr int PARTS = parts_of<T>(), TR = 16 * QB, RS = D + 4;
   __shared__ __attribute__((aligned(16))) float lds[split_lds_floats<QB, NW>()];
   float* s_m = lds + NW * TR * RS;
@@ -781,23 +783,23 @@ static int key_splits(long blocks, int visible, int num_cus) {
 
 // The form of a bfloat16 launch at heads of 64 and 128: the one whose time is the least by an estimate, rounds of blocks (`more`
 // for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
-// its steps of 32 keys x a step), in us as fitted to 1,150 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
+// its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
-// the picks lose 0.7 % (heads of 64) and 1 % (128) to the best of all, 20 % at worst (200 others: 1.3 %, 15 %).  Up to 16 rows a tile's keys are
-// split over waves and blocks; of more rows so, too, where they are few and the keys many.
-// us, split / 2x4 / 2x2 / 4x1, heads of 128: 25 rows of 456 (request, kv head) pairs and 182 keys
-// 17.9 / 18.0 / 12.0 / 15.2; 336 rows of 24 behind 3,300 67 / 38 / 48 / 86; 36 of 4 behind 3,000 13 / 33 / 44 / 77; 3,216 of 4
-// and 536 20 / 14.5 / 14.2 / 21; 12,296 of 6 behind 768 134 / 84 / 63 / 59; 2,176 of 120 and 317 270 / 152 / 85 / 74.
+// the picks lose 0.7 % (heads of 64) and 0.9 % (128) to the best of all (200 others: 1.3 %, 31 % at worst).  Up to 16 rows a
+// tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
+// us, split / 2x4 / 2x2 / 4x1, heads of 128: 48 rows of 56 (request, kv head) pairs behind 6,732 keys 42 / 67 / 92 / 166; 126
+// of 92 behind 881 23.0 / 19.7 / 20.6 / 30.7; 504 of 44 behind 157 18 / 22 / 14 / 15.5; 7,990 of 8 and 1,598 keys 68 / 63 / 47 / 51;
+// 1,368 of 64 behind 309 61 / 70 / 47 / 44; 5,624 of 48 and 712 keys 163 / 188 / 113 / 104.
 enum { FORM_SPLIT = 1, FORM_2x4, FORM_2x2, FORM_4x1 };
 #if STAGED
 static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
   if (most_rows <= 16) return FORM_SPLIT;
   struct Form { int rows, groups; float blocks_a_unit, start, step, more, least; };
-  constexpr Form forms[] = {{32, SPLIT_WAVES, 2.f, D == 64 ? 4.95f : 9.5f, D == 64 ? 1.05f : 2.1f, D == 64 ? .66f : .57f, D == 64 ? 1.f : .7f},
-                            {64, 4, 1.f, D == 64 ? 5.3f : 7.8f, D == 64 ? .9f : 1.27f, .5f, D == 64 ? 1.1f : 1.f},
-                            {64, 2, D == 64 ? 3.f : 2.f, D == 64 ? 5.8f : 7.9f, .9f, D == 64 ? .58f : .65f, D == 64 ? .93f : .84f},
-                            {128, 1, D == 64 ? 3.f : 2.f, D == 64 ? 6.9f : 9.2f, D == 64 ? .72f : .79f, .74f, .9f}};
-  constexpr float MERGE = D == 64 ? 2.7f : 1.9f;
+  constexpr Form forms[] = {{32, SPLIT_WAVES, 2.f, D == 64 ? 4.2f : 6.f, D == 64 ? .92f : 1.38f, D == 64 ? .6f : .67f, D == 64 ? 1.06f : .91f},
+                            {64, 4, 1.f, D == 64 ? 5.f : 8.2f, D == 64 ? .8f : 1.36f, D == 64 ? .65f : .42f, D == 64 ? 1.17f : .92f},
+                            {64, 2, D == 64 ? 3.f : 2.f, D == 64 ? 6.f : 8.2f, D == 64 ? .74f : .93f, D == 64 ? .73f : .67f, D == 64 ? .88f : .83f},
+                            {128, 1, D == 64 ? 3.f : 2.f, D == 64 ? 6.f : 10.5f, D == 64 ? .7f : .84f, D == 64 ? .89f : .67f, D == 64 ? .94f : .87f}};
+  constexpr float MERGE = D == 64 ? 3.9f : 1.8f;
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 4; ++i) {
