@@ -8,16 +8,19 @@
 // times the whole.  The tokens so produced are distributed as the target model's own.  Temperature 0: x_j stands
 // while it is the row's argmax (ties to the smallest index), and the next token is the argmax of the row that is reached.
 //
-// Exponentials and sums are taken in 64 bits (the vector unit runs float64 at the float32 rate and the rows' reading bounds
-// the pass): the running sum of 150,000 weights has a border every 1e-5 or so, and float32 sums taken in another order
-// would cross one in every few hundred draws.  What is summed is summed in one fixed order.
+// Exponentials and sums are taken in 64 bits (the vector unit runs float64 at the float32 rate): the running sum of 150,000
+// weights has a border every 1e-5 or so, and float32 sums taken in another order would cross one in every few hundred
+// draws.  What is summed is summed in one fixed order.
 //
 // Two launches: the rows in chunks (each leaves its maximum, its place and its sum of exponentials), then a block for every
 // chunk of every request's reached row, which finds that row from the chunks' sums, weighs its chunk, and is the one that
-// draws if it is the last of its request.
+// draws if it is the last of its request.  64 requests, 578 rows of 152,064 (351 MB): the first launch takes 68 us (5.2 TB/s; by a
+// polynomial of degree 12 with conversions 89), bound by its exponentials and the reading alike, the second 30: a chain of
+// small steps, 12 us for one request alone (first rows, sums, weights, the count of blocks, the chunk, the place in it).
 #include "common.h"
 
 constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH;
+constexpr double LOG2_E = 1.44269504088896340736;
 constexpr int NONE = 0x7fffffff;      // the place of a maximum that is not there
 
 struct VerifyArgs {
@@ -39,28 +42,28 @@ struct VerifyArgs {
   int* arrived;              // [n]: chunks weighed so far (the first launch clears it)
 };
 
-// e^x for x <= 0 (minus infinity too) to about a rounding: x = n ln 2 + r, |r| <= ln 2 / 2, Taylor's sum of e^r to the
-// twelfth power (what is left out: r^13 / 13! < 2e-16), times 2^n.
-__device__ __forceinline__ double exp_below(double x) {
-  x = fmax(x, -800.0);
-  const double n = rint(x * 1.4426950408889634074);
-  double r = fma(n, -0.69314718055994528623, x);
-  r = fma(n, -2.3190468138462995584e-17, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+// 2^y for y <= 0 (minus infinity, and what is not a number, too: exactly zero) to 1.1e-12 of itself: y = n + f, |f| <= 1/2, the
+// n by adding 1.5 * 2^52 (its low word then is n), the polynomial of degree 8 that meets 2^f at the nine Chebyshev points of
+// [-1/2, 1/2] (zero among them), and n added to the exponent's bits.  Below 2^-1023 it is zero: f is zero there, the polynomial 1 and
+// its exponent's bits all gone.  (Every step at the rate of a product: a rint, a conversion and an ldexp are slower, and the
+// exponentials bound the first launch.)
+__device__ __forceinline__ double exp2_below(double y) {
+  constexpr double WHOLE = 6755399441055744.0;
+  y = fmax(y, -1023.0);
+  const double t = y + WHOLE, f = y - (t - WHOLE);
+  double p = 1.32552248786688168e-06;
+  p = fma(p, f, 1.53100794022492960e-05);
+  p = fma(p, f, 1.54034558524538382e-04);
+  p = fma(p, f, 1.33334505680006454e-03);
+  p = fma(p, f, 9.61812915940255843e-03);
+  p = fma(p, f, 5.55041094120593270e-02);
+  p = fma(p, f, 2.40226506958129887e-01);
+  p = fma(p, f, 6.93147180545933494e-01);
+  p = fma(p, f, 1.0);
+  return __hiloint2double((int)((unsigned)__double2hiint(p) + ((unsigned)__double2loint(t) << 20)), __double2loint(p));
 }
+// A logit's weight where `most` has weight 1; rate = log2 e over the temperature
+__device__ __forceinline__ double weight(float z, float most, double rate) { return exp2_below(((double)z - (double)most) * rate); }
 
 __device__ __forceinline__ bool bounded(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
@@ -75,8 +78,8 @@ __device__ __forceinline__ int wave_min(int v) {
   return v;
 }
 
-// The thread's numbers of a chunk: places quad * 1024 + 4 * thread + 0 .. 3, in rising order; nothing past the row's end,
-// and what is not a number, is minus infinity.
+// The thread's numbers of a chunk: places quad * 1024 + 4 * thread + 0 .. 3, in rising order; minus infinity past the row's
+// end.  (What is not a number stays so: no maximum takes it, and its weight is zero.)
 __device__ __forceinline__ int place(int j) { return (j >> 2) * 4 * THREADS + 4 * (int)threadIdx.x + (j & 3); }
 __device__ __forceinline__ void load_chunk(const float* z, int count, float (&v)[EACH]) {
   if (((uintptr_t)z & 15) == 0 && count == CHUNK) {
@@ -90,8 +93,6 @@ __device__ __forceinline__ void load_chunk(const float* z, int count, float (&v)
 #pragma unroll
     for (int j = 0; j < EACH; ++j) v[j] = place(j) < count ? z[place(j)] : -__builtin_huge_valf();
   }
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) v[j] = v[j] == v[j] ? v[j] : -__builtin_huge_valf();
 }
 
 // The first launch: one chunk of one row (target rows, then the drafting model's).
@@ -115,21 +116,21 @@ __global__ __launch_bounds__(THREADS) void verify_chunks_kernel(VerifyArgs a) {
   }
   const float t = before > 0 ? a.temperature[before - 1] : 0.f;
   if (!target && !(t > 0.f)) return;
-  float most = v[0];
-  int best = 0;
+  float most = -__builtin_huge_valf();
 #pragma unroll
-  for (int j = 1; j < EACH; ++j)
-    if (v[j] > most) {
-      most = v[j];
-      best = j;
-    }
+  for (int j = 0; j < EACH; ++j) most = fmaxf(most, v[j]);
   const float top = full_wave_max(most);
-  const int at_best = wave_min(most == top && top > -__builtin_huge_valf() ? first + place(best) : NONE);
+  int at_best = NONE;
   double sum = 0.0;
-  if (t > 0.f && bounded(top)) {
-    const double inv_t = 1.0 / (double)t;
+  if (!(t > 0.f)) {      // (only the argmax is asked for)
+    int best = EACH;
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) sum += exp_below(((double)v[j] - (double)top) * inv_t);
+    for (int j = EACH - 1; j >= 0; --j) best = v[j] == top ? j : best;
+    at_best = wave_min(best < EACH && top > -__builtin_huge_valf() ? first + place(best) : NONE);
+  } else if (bounded(top)) {
+    const double rate = LOG2_E / (double)t;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) sum += weight(v[j], top, rate);
     sum = wave_sum64(sum);
   }
   if (lane == 0) {
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(THREADS) void verify_chunks_kernel(VerifyArgs a) {
   double total = 0.0;
   for (int w = 0; w < THREADS / 64; ++w) {
     if (s_most[w] == all) place_of = min(place_of, s_best[w]);
-    if (t > 0.f && bounded(all) && bounded(s_most[w])) total += s_sum[w] * exp_below(((double)s_most[w] - (double)all) / (double)t);
+    if (t > 0.f && bounded(all) && bounded(s_most[w])) total += s_sum[w] * weight(s_most[w], all, LOG2_E / (double)t);
   }
   const size_t at = (size_t)row * a.chunks + chunk;
   a.most[at] = all;
@@ -159,7 +160,7 @@ struct RowSum {
   double sum;
 };
 // A row's chunks put together, by one wave; every lane gets the result
-__device__ __forceinline__ RowSum whole_row(const VerifyArgs& a, int row, double inv_t) {
+__device__ __forceinline__ RowSum whole_row(const VerifyArgs& a, int row, double rate) {
   const size_t at = (size_t)row * a.chunks;
   const int lane = threadIdx.x & 63;
   float most = -__builtin_huge_valf();
@@ -170,17 +171,17 @@ __device__ __forceinline__ RowSum whole_row(const VerifyArgs& a, int row, double
     const int i = a.best[at + c];
     const double s = a.sum[at + c];
     if (m > most) {      // (a lane's chunks: the running sum in units of the running maximum)
-      sum = bounded(most) && bounded(m) ? sum * exp_below(((double)most - (double)m) * inv_t) + s : s;
+      sum = bounded(most) && bounded(m) ? sum * weight(most, m, rate) + s : s;
       most = m;
       best = i;
     } else if (bounded(m) && bounded(most)) {
-      sum += s * exp_below(((double)m - (double)most) * inv_t);
+      sum += s * weight(m, most, rate);
     }
   }
   RowSum r;
   r.most = full_wave_max(most);
   r.best = wave_min(most == r.most ? best : NONE);
-  r.sum = wave_sum64(bounded(most) && bounded(r.most) ? sum * exp_below(((double)most - (double)r.most) * inv_t) : 0.0);
+  r.sum = wave_sum64(bounded(most) && bounded(r.most) ? sum * weight(most, r.most, rate) : 0.0);
   return r;
 }
 
@@ -189,7 +190,7 @@ struct Source {
   int row, draft_row;        // the row, the draft's that is subtracted (-1: none)
   int without;               // the token that has no weight (a draft without logits that fell), or -1
   float most, draft_most;
-  double inv_t, inv_sum, draft_inv_sum;
+  double rate, inv_sum, draft_inv_sum;
 };
 
 __device__ __forceinline__ void chunk_weights(const VerifyArgs& a, const Source& d, int first, double (&w)[EACH]) {
@@ -198,14 +199,14 @@ __device__ __forceinline__ void chunk_weights(const VerifyArgs& a, const Source&
   load_chunk(a.logits + (size_t)d.row * a.stride + first, count, z);
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
-    w[j] = exp_below(((double)z[j] - (double)d.most) * d.inv_t) * d.inv_sum;
+    w[j] = weight(z[j], d.most, d.rate) * d.inv_sum;
     if (first + place(j) == d.without) w[j] = 0.0;
   }
   if (d.draft_row < 0) return;
   load_chunk(a.draft + (size_t)d.draft_row * a.draft_stride + first, count, z);
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
-    const double q = exp_below(((double)z[j] - (double)d.draft_most) * d.inv_t) * d.draft_inv_sum;
+    const double q = weight(z[j], d.draft_most, d.rate) * d.draft_inv_sum;
     w[j] = w[j] > q ? w[j] - q : 0.0;
   }
 }
@@ -226,14 +227,15 @@ __device__ __forceinline__ double running_sum(double v) {
 template <typename F>
 __device__ __forceinline__ int pick_chunk(int chunks, double u, F mass, double* left) {
   const int lane = threadIdx.x & 63;
-  double total = 0.0;
-  for (int base = 0; base < chunks; base += 64) total += __shfl(running_sum(base + lane < chunks ? mass(base + lane) : 0.0), 63, WAVE);
+  const double first = lane < chunks ? mass(lane) : 0.0;
+  double total = __shfl(running_sum(first), 63, WAVE);
+  for (int base = 64; base < chunks; base += 64) total += __shfl(running_sum(base + lane < chunks ? mass(base + lane) : 0.0), 63, WAVE);
   if (!(total > 0.0)) return -1;
   const double target = u * total;
   double run = 0.0;
   int chunk = -1;
   for (int base = 0; base < chunks; base += 64) {
-    const double m = base + lane < chunks ? mass(base + lane) : 0.0;
+    const double m = base == 0 ? first : base + lane < chunks ? mass(base + lane) : 0.0;
     const double sum = run + running_sum(m);
     const unsigned long long positive = __ballot(m > 0.0), reached = __ballot(m > 0.0 && sum >= target);
     const unsigned long long use = reached ? reached & -reached : 0;
@@ -251,40 +253,18 @@ __device__ __forceinline__ int pick_chunk(int chunks, double u, F mass, double* 
 // The second launch: a block for every (chunk, request).
 __global__ __launch_bounds__(THREADS) void verify_draw_kernel(VerifyArgs a) {
   constexpr int WAVES = THREADS / 64;
-  __shared__ int s_first, s_last, s_chunk, s_wave_last[WAVES];
+  constexpr int AT_ONCE = 16;      // drafted tokens looked at together
+  __shared__ int s_last, s_chunk, s_plain;
   __shared__ double s_sum[WAVES], s_left;
+  __shared__ RowSum s_row[2 * AT_ONCE + 1];
   const int chunk = blockIdx.x, b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r0 = a.row_start[b];
   int count = a.row_start[b + 1] - r0;
+  const float t = a.temperature[b];
   // (a request without a row, or starts that do not fit the rows: no token)
   if (count < 1 || r0 < b || count > a.rows - r0 || count - 1 > a.rows - a.n - (r0 - b)) count = 0;
-  const float t = a.temperature[b];
   const bool greedy = !(t > 0.f);
   if ((greedy || count == 0) && chunk > 0) return;
-  const double inv_t = greedy ? 0.0 : 1.0 / (double)t;
-
-  // which drafted tokens stand: the first that falls (or the last row)
-  if (threadIdx.x == 0) s_first = max(count - 1, 0);
-  __syncthreads();
-  for (int j = wave; j < count - 1; j += WAVES) {
-    const int x = a.drafts[r0 - b + j];
-    const RowSum p = whole_row(a, r0 + j, inv_t);
-    bool stands = x >= 0 && x < a.vocab;
-    if (greedy) {
-      stands = x == p.best;
-    } else if (stands) {
-      const double px = exp(((double)a.logits[(size_t)(r0 + j) * a.stride + x] - (double)p.most) * inv_t) / p.sum;
-      double qx = 1.0;
-      if (a.draft) {
-        const RowSum q = whole_row(a, a.rows + r0 - b + j, inv_t);
-        qx = exp(((double)a.draft[(size_t)(r0 - b + j) * a.draft_stride + x] - (double)q.most) * inv_t) / q.sum;
-      }
-      stands = (double)a.uniform[r0 + j] * qx < px;      // (false where either is not a number)
-    }
-    if (!stands && lane == 0) atomicMin(&s_first, j);
-  }
-  __syncthreads();
-  const int first = s_first;
   if (count == 0) {
     if (threadIdx.x == 0) {
       a.accepted[b] = 0;
@@ -292,14 +272,67 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(VerifyArgs a) {
     }
     return;
   }
+  const double rate = greedy ? 0.0 : LOG2_E / (double)t;
 
-  // the row that is reached (every wave the same)
-  const RowSum p = whole_row(a, r0 + first, inv_t);
-  Source d{r0 + first, -1, -1, p.most, 0.f, inv_t, 1.0 / p.sum, 0.0};
+  // Which drafted tokens stand: the first that falls, or the last row.  A wave a row of logits; then every wave, a lane a token, all alike.
+  const bool with_draft = a.draft != nullptr && !greedy;
+  int first = count - 1;
+  RowSum p = {}, q = {};
+  for (int from = 0;; from += AT_ONCE) {
+    const int n = min(AT_ONCE, count - 1 - from), rows = with_draft ? 2 * n : n;
+    const bool at_end = from + n == count - 1;
+    const int j = from + min(lane, max(n - 1, 0));
+    // (asked for before the sums)
+    int x = -1;
+    float zx = 0.f, dx = 0.f, u = 0.f;
+    if (lane < n) {
+      x = a.drafts[r0 - b + j];
+      u = a.uniform[r0 + j];
+      if (x >= 0 && x < a.vocab) {
+        zx = a.logits[(size_t)(r0 + j) * a.stride + x];
+        if (with_draft) dx = a.draft[(size_t)(r0 - b + j) * a.draft_stride + x];
+      }
+    }
+    for (int i = wave; i < rows + (at_end ? 1 : 0); i += WAVES) {
+      const int of = i == rows ? n : i < n ? i : i - n;
+      const RowSum r = whole_row(a, i < n || i == rows ? r0 + from + of : a.rows + r0 - b + from + of, rate);
+      if (lane == 0) s_row[i == rows ? 2 * AT_ONCE : i < n ? i : AT_ONCE + of] = r;
+    }
+    __syncthreads();
+    bool stands = lane >= n;
+    if (lane < n && x >= 0 && x < a.vocab) {
+      const RowSum of_p = s_row[lane];
+      if (greedy) {
+        stands = x == of_p.best;
+      } else {
+        double qx = 1.0;
+        if (with_draft) {
+          const RowSum of_q = s_row[AT_ONCE + lane];
+          qx = bounded(of_q.most) ? weight(dx, of_q.most, rate) / of_q.sum : __builtin_nan("");
+        }
+        const double px = bounded(of_p.most) ? weight(zx, of_p.most, rate) / of_p.sum : 0.0;
+        stands = (double)u * qx < px;      // (false where either is not a number)
+      }
+    }
+    const unsigned long long falls = ~__ballot(stands);
+    if (falls) {
+      const int at = __ffsll(falls) - 1;
+      first = from + at;
+      p = s_row[at];
+      if (with_draft) q = s_row[AT_ONCE + at];
+      break;
+    }
+    if (at_end) {
+      p = s_row[2 * AT_ONCE];
+      break;
+    }
+    __syncthreads();
+  }
+
+  Source d{r0 + first, -1, -1, p.most, 0.f, rate, 1.0 / p.sum, 0.0};
   bool sound = greedy ? p.best != NONE : bounded(p.most);
   if (!greedy && first < count - 1) {
     if (a.draft) {
-      const RowSum q = whole_row(a, a.rows + r0 - b + first, inv_t);
       d.draft_row = r0 - b + first;
       d.draft_most = q.most;
       d.draft_inv_sum = 1.0 / q.sum;
@@ -344,72 +377,80 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(VerifyArgs a) {
       plain = 1;
       const size_t of = (size_t)d.row * a.chunks;
       at = pick_chunk(a.chunks, u, [&](int c) {
-        return bounded(a.most[of + c]) ? a.sum[of + c] * exp_below(((double)a.most[of + c] - (double)d.most) * inv_t) * d.inv_sum : 0.0;
+        return bounded(a.most[of + c]) ? a.sum[of + c] * weight(a.most[of + c], d.most, rate) * d.inv_sum : 0.0;
       }, &left);
     }
     if (lane == 0) {
       s_chunk = at;
       s_left = left;
-      s_first = plain;
+      s_plain = plain;
     }
   }
   __syncthreads();
-  if (s_first) d.draft_row = d.without = -1;
+  if (s_plain) d.draft_row = d.without = -1;
   const int from = s_chunk * CHUNK;
   if (s_chunk < 0) {
     if (threadIdx.x == 0) a.tokens[b] = -1;
     return;
   }
-  // The place in the chunk.  Its places in rising order are quad after quad of 1,024, in each thread after thread: the running sum over
-  // the threads' sums of four, quad by quad.
+  // The place in the chunk.  Its places in rising order are quad after quad of 1,024, in each wave after wave, thread after thread: the
+  // running sum over the threads' sums of four.
   chunk_weights(a, d, from, w);
-  double run = 0.0;
+  constexpr int QUADS = EACH / 4, PARTS = QUADS * WAVES;
+  __shared__ double s_part[PARTS];
+  __shared__ int s_has[PARTS], s_reached[PARTS];      // the last lane with weight, the first that reaches what is left (-1: none)
   const double left = s_left;
-  int last_positive = -1;
-  for (int q = 0; q < EACH / 4; ++q) {
-    const double four = (w[4 * q] + w[4 * q + 1]) + (w[4 * q + 2] + w[4 * q + 3]);
-    const double sum = running_sum(four);
-    const unsigned long long positive = __ballot(four > 0.0);
-    __syncthreads();
-    if (lane == 63) s_sum[wave] = sum;
-    if (lane == 0) s_wave_last[wave] = positive ? 63 - __clzll(positive) : -1;
-    __syncthreads();
-    double before = run;
-    for (int i = 0; i < wave; ++i) before += s_sum[i];
-    for (int i = 0; i < WAVES; ++i) {
-      run += s_sum[i];
-      if (s_wave_last[i] >= 0) last_positive = q * THREADS + i * 64 + s_wave_last[i];
-    }
-    // the first thread whose sum reaches what is left
-    const unsigned long long reached = __ballot(four > 0.0 && before + sum >= left);
-    if (lane == 0) s_wave_last[wave] = reached ? __ffsll(reached) - 1 : -1;
-    __syncthreads();
-    int owner = -1;
-    for (int i = WAVES - 1; i >= 0; --i)
-      if (s_wave_last[i] >= 0) owner = i * 64 + s_wave_last[i];
-    if (owner < 0) continue;
-    if ((int)threadIdx.x == owner) {
-      double r = before + (sum - four);
-      int token = -1;
+  double four[QUADS], sum[QUADS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (token >= 0 && r >= left) break;
-        if (w[4 * q + j] > 0.0) token = from + place(4 * q + j);
-        r += w[4 * q + j];
+  for (int k = 0; k < QUADS; ++k) {
+    four[k] = (w[4 * k] + w[4 * k + 1]) + (w[4 * k + 2] + w[4 * k + 3]);
+    sum[k] = running_sum(four[k]);
+    const unsigned long long positive = __ballot(four[k] > 0.0);
+    if (lane == 63) s_part[k * WAVES + wave] = sum[k];
+    if (lane == 0) s_has[k * WAVES + wave] = positive ? 63 - __clzll(positive) : -1;
+  }
+  __syncthreads();
+  double before = 0.0;
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    if (i % WAVES == wave) {
+      const int k = i / WAVES;
+      sum[k] += before;
+      const unsigned long long reached = __ballot(four[k] > 0.0 && sum[k] >= left);
+      if (lane == 0) s_reached[i] = reached ? __ffsll(reached) - 1 : -1;
+    }
+    before += s_part[i];
+  }
+  __syncthreads();
+  int part = -1, owner = 0;
+  bool whole = false;      // roundings kept the sum short of it: the last token that has weight
+  for (int i = PARTS - 1; i >= 0; --i)
+    if (s_reached[i] >= 0) {
+      part = i;
+      owner = s_reached[i];
+    }
+  if (part < 0) {
+    whole = true;
+    for (int i = 0; i < PARTS; ++i)
+      if (s_has[i] >= 0) {
+        part = i;
+        owner = s_has[i];
       }
-      a.tokens[b] = token;
-    }
-    return;
   }
-  // (roundings kept the sum short of it: the last token that has weight)
-  if (last_positive >= 0 && (int)threadIdx.x == last_positive % THREADS) {
-    const int q = last_positive / THREADS;
-    int token = -1;
+  if (part < 0 || part % WAVES != wave || lane != owner) return;
+  int token = -1;
 #pragma unroll
-    for (int j = 0; j < EACH; ++j)
-      if ((j >> 2) == q && w[j] > 0.0) token = from + place(j);
-    a.tokens[b] = token;
+  for (int k = 0; k < QUADS; ++k) {
+    if (k != part / WAVES) continue;
+    double run = sum[k] - four[k];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!whole && token >= 0 && run >= left) break;
+      if (w[4 * k + j] > 0.0) token = from + place(4 * k + j);
+      run += w[4 * k + j];
+    }
   }
+  a.tokens[b] = token;
 }
 
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
