@@ -65,6 +65,7 @@ struct Args {
   void* out;                   // [rows, out_stride]
   long q_stride, out_stride;
   int table_stride, table_width, page_shift, pages;
+  int last_key;                // the last that the table has room for
   int nq, nkv, window, rows, reqs, splits;
   float scale2;                // the scores' factor times log2 e
   float* o_part;               // [rows * nq, splits, D]    (splits > 1)
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attention_e4m3_spli
   const int first_pos = before + row0 / G, key_hi = before + last / G;
   const int key_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
   const int full_lo = a.window > 0 ? max(0, key_hi - a.window + 1) : 0;      // from here on every row sees a key before first_pos
-  const int step_lo = key_lo >> 5, step_hi = (key_hi >> 5) + 1;
+  const int step_lo = key_lo >> 5, step_hi = (min(key_hi, a.last_key) >> 5) + 1;
   const int per = (step_hi - step_lo + a.splits - 1) / a.splits;
   const int blk_lo = step_lo + part * per, blk_hi = min(blk_lo + per, step_hi);
   const int per_wave = (max(blk_hi - blk_lo, 0) + NW - 1) / NW;
@@ -473,8 +474,8 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
   const int last = min(row0 + 32, total) - 1, block_last = min(block_row0 + RT * 32, total) - 1;
   const int p_first = before + row0 / G, p_last = row0 < total ? before + last / G : -1;
   const int full_lo = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
-  const int key_hi = max(before + block_last / G, 0);
-  const int key_lo = a.window > 0 ? max(0, before + block_row0 / G - a.window + 1) : 0;
+  const int key_hi = max(min(before + block_last / G, a.last_key), 0);
+  const int key_lo = a.window > 0 ? min(max(0, before + block_row0 / G - a.window + 1), key_hi) : 0;
   const int tile_lo = key_lo / KT, tile_hi = key_hi / KT;
   const int block_lo = key_lo & ~15, block_hi = key_hi & ~15;
 
@@ -490,10 +491,10 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
   auto locate = [&](int from) {
     base = from;
     auto block_at = [&](int block16, bool of_scales) {
-      const int key = max(min(min(from + lane, tile_hi) * KT + block16 * 16, block_hi), block_lo), at = key >> shift;
+      const int own = min(from + lane, tile_hi) * KT + block16 * 16, key = max(min(own, block_hi), block_lo), at = key >> shift;
       int page = -1;
       if (a.table_width > 0) page = table_entry(table, min(at, a.table_width - 1));
-      const bool there = at < a.table_width && page >= 0 && page < a.pages;
+      const bool there = own <= block_hi && at < a.table_width && page >= 0 && page < a.pages;
       const unsigned row = (unsigned)(there ? page : 0) * a.nkv + kvh;
       return (row * (of_scales ? 2 : 1) * page_blocks + ((key >> 4) & (page_blocks - 1))) | (there ? 0u : ~HERE);
     };
@@ -866,10 +867,11 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
                  "attention(e4m3): the pages are not aligned for vector loads");
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;
   Args a{q, (const unsigned char*)k, (const unsigned char*)v, (const unsigned char*)kv_scale, table, q_start, start_pos, out,
-         q_stride, out_stride, table_stride, table_width, 0, pages, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
+         q_stride, out_stride, table_stride, table_width, 0, pages,
+         (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
          nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
-  const long most_rows = (long)max_q_len * (nq / nkv);
+  const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
   const int visible = window > 0 ? (int)std::min((long)max_ctx_len, (long)window + max_q_len) : max_ctx_len;
   if (num_cus <= 0) num_cus = 256;
   if (dtype == DT_F32)

@@ -87,3 +87,22 @@ def test_the_same_every_time(ops, form):      # noqa: F811
     with ops.debug.force(e4m3_attention=(d, 0, form)):
         outs = [run(ops, cache, q, nq, q_start, start_pos, lengths, counts, None, 1 / math.sqrt(d) / 64, dev=dev) for _ in range(4)]
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("form", [0] + FORMS)
+def test_positions_beyond_the_table(ops, form):      # noqa: F811
+    """Rows far behind what the table has room for see what it has, and no walk goes further."""
+    nq, nkv, d, page = 4, 2, 64, 16
+    cache = Cache([80], nkv, d, page).fill()
+    q = queries(33, nq, d, "bf16", 1)
+    far = torch.tensor([1 << 30], dtype=torch.int32)
+    with ops.debug.force(e4m3_attention=(d, 0, form)):
+        got = run(ops, cache, q, nq, torch.tensor([0, 33], dtype=torch.int32), far, [80], [33], None, 0.002)
+        gone = run(ops, cache, q, nq, torch.tensor([0, 33], dtype=torch.int32), far, [80], [33], 50, 0.002)
+    one = torch.tensor([79], dtype=torch.int32)
+    for i in (0, 17, 32):
+        want, spread, reach = plain.attention(q[i:i + 1], nq, nkv, d, cache.k, cache.v, cache.scale, cache.table, page,
+                                              torch.tensor([0, 1], dtype=torch.int32), one, 1, None, 0.002)
+        tol = plain.tolerance(torch.bfloat16, want, spread, reach, 80, d)
+        assert bool(((got[i].double().view(1, nq, d) - want).abs() <= tol).all())
+    assert not bool(gone.any())
