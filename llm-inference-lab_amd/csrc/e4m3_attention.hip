@@ -775,10 +775,12 @@ extern "C" void llmlab_debug_attention_e4m3(int splits, int form) {
 }
 
 constexpr int SPLIT_WAVES = 4;
-// Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys.
+// Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys, and none of
+// up to 32 steps, where the launch that puts the splits together costs what they gain (one to 16 requests of 28 heads of 128 over 4 at 700
+// to 1,000 keys 8.3 to 10.5 us of GPU in one launch, 8.5 to 10.2 in two, and the host 2.5 us less; at 1,500 12.1 and 9.2).
 static int key_splits(long blocks, int visible, int num_cus) {
-  if (blocks >= num_cus) return 1;
   const long steps = (visible + 31) / 32, most = (steps + 7) / 8;
+  if (blocks >= num_cus || steps <= 32) return 1;
   return (int)std::max(1L, std::min(std::min(2L * num_cus / blocks, most), 128L));
 }
 

@@ -40,6 +40,7 @@ def _dt(t: torch.Tensor) -> int:
     raise TypeError(f"kernels take float32 or bfloat16 tensors, got {t.dtype}")
 
 
+_E4M3 = torch.float8_e4m3fn
 _DTYPE_CODES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 
 
@@ -1130,14 +1131,27 @@ class HipOps:
         self._e4m3_attention_lib(head_dim)
         self._mixer_lib("e4m3_cache")
 
-    def _e4m3_pages(self, what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table) -> None:
+    def _e4m3_pages(self, what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table):
+        """The checks of a cache of 8 bits; its three addresses.  (In one expression first: a call of a decode step is bound by
+        what the host does for it, and the checks one by one were a third of that.)"""
+        pages = k_cache.shape[0]
+        keys, values, scales = k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr()
+        where = self.device
+        if (k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3 and kv_scale.dtype is torch.uint8 and block_table.dtype is torch.int32
+                and k_cache.device == where and v_cache.device == where and kv_scale.device == where and block_table.device == where
+                and k_cache.is_contiguous() and v_cache.is_contiguous() and kv_scale.is_contiguous()
+                and k_cache.shape == (pages, num_kv_heads, page_size, head_dim)
+                and v_cache.shape == (pages, num_kv_heads, head_dim, page_size)
+                and kv_scale.shape == (pages, num_kv_heads, 2, page_size) and not (keys | values | scales) & 15
+                and page_size >= 16 and not page_size & (page_size - 1) and not head_dim & 15 and 16 <= head_dim <= 256
+                and block_table.dim() == 2 and block_table.is_contiguous()):
+            return keys, values, scales
         if page_size < 16 or page_size & (page_size - 1):
             raise UnsupportedSizeError(f"page size {page_size} is not a power of two >= 16")
         if head_dim % 16 or not 16 <= head_dim <= 256:
             raise UnsupportedSizeError(f"{what}: head sizes are multiples of 16 from 16 to 256, got {head_dim}")
-        pages = k_cache.shape[0]
-        for t, name, dtype, shape in ((k_cache, "keys", torch.float8_e4m3fn, (pages, num_kv_heads, page_size, head_dim)),
-                                      (v_cache, "values", torch.float8_e4m3fn, (pages, num_kv_heads, head_dim, page_size)),
+        for t, name, dtype, shape in ((k_cache, "keys", _E4M3, (pages, num_kv_heads, page_size, head_dim)),
+                                      (v_cache, "values", _E4M3, (pages, num_kv_heads, head_dim, page_size)),
                                       (kv_scale, "scales", torch.uint8, (pages, num_kv_heads, 2, page_size))):
             self._need(t, f"{what}: cached {name}", dtype)
             if tuple(t.shape) != shape:
@@ -1147,12 +1161,17 @@ class HipOps:
         self._need(block_table, "block table", torch.int32, contiguous=False)
         if block_table.dim() != 2 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
             raise ValueError(f"{what}: the block table has a row of page numbers per request")
+        return keys, values, scales
 
     def _rows_of(self, what, positions, row_req, rows) -> None:
-        self._need(positions, "positions", torch.int32)
-        self._need(row_req, "row -> request map", torch.int32)
+        self._need_int32(positions, "positions")
+        self._need_int32(row_req, "row -> request map")
         if positions.numel() < rows or row_req.numel() < rows:
             raise ValueError(f"{what}: one position and one request index per row")
+
+    def _need_int32(self, t, name) -> None:
+        if t.dtype is not torch.int32 or t.device != self.device or not t.is_contiguous():
+            self._need(t, name, torch.int32)
 
     def rope_kv_write_e4m3(self, qkv, num_heads, num_kv_heads, head_dim, inv_freq, positions, row_req, block_table, page_size,
                            k_cache, v_cache, kv_scale, q_out) -> None:
@@ -1169,26 +1188,33 @@ class HipOps:
         has no page in its request's row of the table stores nothing.  Two rows of one call may not name the same position of
         the same request."""
         what = "rope_kv_write_e4m3"
-        _dt(qkv)
-        self._need(qkv, "qkv", contiguous=False)
-        rows = qkv.shape[0]
-        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
-            raise ValueError(f"{what}: qkv {tuple(qkv.shape)} does not hold {num_heads}+2*{num_kv_heads} heads of {head_dim}")
-        self._need(q_out, "queries", qkv.dtype, contiguous=False)
-        if tuple(q_out.shape) != (rows, num_heads * head_dim) or q_out.stride(1) != 1:
-            raise ValueError(f"{what}: queries {tuple(q_out.shape)} for {rows} rows of {num_heads} heads of {head_dim}")
+        kind, where = _dt(qkv), self.device
+        shape, q_shape = qkv.shape, q_out.shape
+        rows, strides, q_strides = shape[0], qkv.stride(), q_out.stride()
+        if not (qkv.device == where and q_out.device == where and q_out.dtype is qkv.dtype
+                and shape == (rows, (num_heads + 2 * num_kv_heads) * head_dim) and strides[1] == 1
+                and q_shape == (rows, num_heads * head_dim) and q_strides[1] == 1):
+            self._need(qkv, "qkv", contiguous=False)
+            if qkv.dim() != 2 or strides[1] != 1 or shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
+                raise ValueError(f"{what}: qkv {tuple(shape)} does not hold {num_heads}+2*{num_kv_heads} heads of {head_dim}")
+            self._need(q_out, "queries", qkv.dtype, contiguous=False)
+            raise ValueError(f"{what}: queries {tuple(q_shape)} for {rows} rows of {num_heads} heads of {head_dim}")
         self._rows_of(what, positions, row_req, rows)
+        turn = None
         if inv_freq is not None:
-            self._need(inv_freq, "rotary frequencies", torch.float32)
+            if inv_freq.dtype is not torch.float32 or inv_freq.device != where or not inv_freq.is_contiguous():
+                self._need(inv_freq, "rotary frequencies", torch.float32)
             if inv_freq.numel() != head_dim // 2:
                 raise ValueError(f"{what}: the frequency table must hold head_dim/2 entries")
-        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+            turn = inv_freq.data_ptr()
+        keys, values, scales = self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
         lib = self._mixer_lib("e4m3_cache")
-        self._call(lib.llmlab_rope_kv_write_e4m3, self._ptr(qkv), _dt(qkv), rows, qkv.stride(0) if rows > 1 else qkv.shape[1],
-                   num_heads, num_kv_heads, head_dim, self._ptr(inv_freq), self._ptr(positions), self._ptr(row_req),
-                   self._ptr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], page_size,
-                   k_cache.shape[0], self._ptr(k_cache), self._ptr(v_cache), self._ptr(kv_scale), self._ptr(q_out),
-                   q_out.stride(0) if rows > 1 else q_out.shape[1], self._stream(), lib=lib)
+        reqs, width = block_table.shape
+        self._call(lib.llmlab_rope_kv_write_e4m3, qkv.data_ptr(), kind, rows, strides[0] if rows > 1 else shape[1],
+                   num_heads, num_kv_heads, head_dim, turn, positions.data_ptr(), row_req.data_ptr(),
+                   block_table.data_ptr(), block_table.stride(0), width, reqs, page_size,
+                   k_cache.shape[0], keys, values, scales, q_out.data_ptr(),
+                   q_strides[0] if rows > 1 else q_shape[1], self._stream(), lib=lib)
 
     def read_kv_e4m3(self, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, positions, row_req, block_table, page_size,
                      k_out, v_out) -> None:
@@ -1198,20 +1224,23 @@ class HipOps:
         what = "read_kv_e4m3"
         rows = k_out.shape[0]
         _dt(k_out)
-        self._need(k_out, "keys read back")
-        self._need(v_out, "values read back", k_out.dtype)
-        for t in (k_out, v_out):
-            if tuple(t.shape) != (rows, num_kv_heads * head_dim):
-                raise ValueError(f"{what}: output {tuple(t.shape)} for {rows} rows of {num_kv_heads} heads of {head_dim}")
-            if t.data_ptr() % 16:
-                raise ValueError(f"{what}: outputs are not aligned to 16 bytes")
+        keys_out, values_out = k_out.data_ptr(), v_out.data_ptr()
+        shape = (rows, num_kv_heads * head_dim)
+        if not (k_out.device == self.device and v_out.device == self.device and v_out.dtype is k_out.dtype and k_out.is_contiguous()
+                and v_out.is_contiguous() and k_out.shape == shape and v_out.shape == shape and not (keys_out | values_out) & 15):
+            self._need(k_out, "keys read back")
+            self._need(v_out, "values read back", k_out.dtype)
+            for t in (k_out, v_out):
+                if tuple(t.shape) != shape:
+                    raise ValueError(f"{what}: output {tuple(t.shape)} for {rows} rows of {num_kv_heads} heads of {head_dim}")
+            raise ValueError(f"{what}: outputs are not aligned to 16 bytes")
         self._rows_of(what, positions, row_req, rows)
-        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+        keys, values, scales = self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
         lib = self._mixer_lib("e4m3_cache")
-        self._call(lib.llmlab_read_kv_e4m3, self._ptr(k_cache), self._ptr(v_cache), self._ptr(kv_scale), num_kv_heads, head_dim,
-                   rows, self._ptr(positions), self._ptr(row_req), self._ptr(block_table), block_table.stride(0),
-                   block_table.shape[1], block_table.shape[0], page_size, k_cache.shape[0], self._ptr(k_out), self._ptr(v_out),
-                   _dt(k_out), self._stream(), lib=lib)
+        reqs, width = block_table.shape
+        self._call(lib.llmlab_read_kv_e4m3, keys, values, scales, num_kv_heads, head_dim, rows, positions.data_ptr(),
+                   row_req.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, reqs, page_size, k_cache.shape[0],
+                   keys_out, values_out, _dt(k_out), self._stream(), lib=lib)
 
     def paged_attention_e4m3(self, q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
                              q_start, start_pos, n_reqs, max_q_len, max_ctx_len, window, scale, out) -> None:
@@ -1233,31 +1262,33 @@ class HipOps:
         what = "attention"
         if num_kv_heads <= 0 or num_heads % num_kv_heads:
             raise UnsupportedSizeError(f"{num_heads} heads are not a multiple of {num_kv_heads} kv heads")
-        self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
+        keys, values, scales = self._e4m3_pages(what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table)
         lib = self._e4m3_attention_lib(head_dim)
-        _dt(q)
-        rows = q.shape[0]
-        self._need(q, "queries", contiguous=False)
-        self._need(out, "attention output", q.dtype)
-        self._need(q_start, "request row starts", torch.int32)
-        self._need(start_pos, "request start positions", torch.int32)
-        if q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1) or q.shape[1] < num_heads * head_dim:
+        kind = _dt(q)
+        shape, strides, width_out = q.shape, q.stride(), num_heads * head_dim
+        rows = shape[0]
+        if q.device != self.device or out.dtype is not q.dtype or out.device != self.device or not out.is_contiguous():
+            self._need(q, "queries", contiguous=False)
+            self._need(out, "attention output", q.dtype)
+        self._need_int32(q_start, "request row starts")
+        self._need_int32(start_pos, "request start positions")
+        if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or shape[1] < width_out:
             raise ValueError("attention: the query rows are too narrow")
-        if tuple(out.shape) != (rows, num_heads * head_dim):
-            raise ValueError(f"attention: output {tuple(out.shape)} != ({rows}, {num_heads * head_dim})")
-        q_stride = q.stride(0) if rows > 1 else q.shape[1]
-        if q.data_ptr() % 16 or out.data_ptr() % 16 or q_stride * q.element_size() % 16:
+        if out.shape != (rows, width_out):
+            raise ValueError(f"attention: output {tuple(out.shape)} != ({rows}, {width_out})")
+        q_stride = strides[0] if rows > 1 else shape[1]
+        q_at, out_at = q.data_ptr(), out.data_ptr()
+        if (q_at | out_at | q_stride * q.element_size()) & 15:
             raise ValueError("attention: queries and output are not aligned to 16 bytes")
         if window is not None and window <= 0:
             raise ValueError(f"attention: a window holds at least the current position, got {window}")
-        args = [self._ptr(q), _dt(q), q_stride, num_heads, num_kv_heads, self._ptr(k_cache), self._ptr(v_cache),
-                self._ptr(kv_scale), k_cache.shape[0], self._ptr(block_table), block_table.stride(0), block_table.shape[1],
-                page_size, self._ptr(q_start), self._ptr(start_pos), 0, 0, 0, int(window) if window else 0, float(scale),
-                self._ptr(out), num_heads * head_dim, rows, self._ptr(self.workspace), self.workspace.numel(), self.num_cus,
-                None]
+        reqs, width = block_table.shape
+        args = [q_at, kind, q_stride, num_heads, num_kv_heads, keys, values, scales, k_cache.shape[0], block_table.data_ptr(),
+                block_table.stride(0), width, page_size, q_start.data_ptr(), start_pos.data_ptr(), 0, 0, 0,
+                int(window) if window else 0, float(scale), out_at, width_out, rows, self.workspace.data_ptr(),
+                self.workspace.numel(), self.num_cus, None]
         return E4m3AttentionCall(self, lib, args,
-                                 most_requests=min(q_start.numel() - 1, start_pos.numel(), block_table.shape[0]),
-                                 most_context=block_table.shape[1] * page_size)
+                                 most_requests=min(q_start.numel() - 1, start_pos.numel(), reqs), most_context=width * page_size)
 
     # ------------------------------------------- layer norm, plain activations
     def layernorm(self, x, weight, eps, out, rows=None) -> None:
