@@ -30,6 +30,7 @@ constexpr int KP = (D + 63) / 64;        // pieces of 64 numbers of a key
 constexpr int DB = D / 16;               // 16-wide blocks of a value
 constexpr int VG = (DB + 3) / 4;         // groups of four of them
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float LARGE = 1.7014118346046923e38f;      // 2^127
 constexpr float LAZY_MAX = 8.f;          // slack of the running maximum, in powers of two (see below)
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
@@ -219,7 +220,8 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
     }
   }
   // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not keep
-  // out of the product: they become zeros, and the rows that do see them become no numbers.
+  // out of the product: they become zeros, and the rows that do see them become no numbers: infinity (a product too large for
+  // float32, where place and row meet) and minus infinity are added to their sums.
   if constexpr (MASKED) {
     bool strange = false;
 #pragma unroll
@@ -227,11 +229,14 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 #pragma unroll
       for (int db = 0; db < DB; ++db) strange |= (((f.v[h2][db] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
     if (__any(strange)) {
-      bf16x8 seen[QB];
+      bf16x8 up[QB], down[QB];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) seen[qb][i] = sees(qb, i) ? (bf16_t)1.f : (bf16_t)0.f;
+        for (int i = 0; i < 8; ++i) {
+          up[qb][i] = sees(qb, i) ? (bf16_t)LARGE : (bf16_t)0.f;
+          down[qb][i] = -up[qb][i];
+        }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         bf16x8 bad;
@@ -239,15 +244,13 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
         for (int i = 0; i < 8; ++i) {
           const unsigned shift = 8 * (i & 3);
           const bool nan = ((f.v[i >> 2][db] >> shift) & 0x7fu) == 0x7fu;
-          bad[i] = nan ? (bf16_t)1.f : (bf16_t)0.f;
+          bad[i] = nan ? (bf16_t)LARGE : (bf16_t)0.f;
           if (nan) f.v[i >> 2][db] &= ~(0xffu << shift);
         }
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-          const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, seen[qb], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hits[i] > 0.f) r.o[qb][db][i] = __builtin_nanf("");
+          r.o[qb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, up[qb], r.o[qb][db], 0, 0, 0);
+          r.o[qb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, down[qb], r.o[qb][db], 0, 0, 0);
         }
       }
     }
@@ -268,8 +271,14 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 template <int QB, int NW>
 constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
 
+// The waves that a SIMD is to hold: as many as fit without a spilled register (a wave more, with five to eight spilled, changed
+// nothing at heads of 64 and 128).
+constexpr int split_waves(int qb, int parts) {
+  if (qb == 1 && parts == 1) return D <= 64 ? 4 : D <= 112 ? 3 : D <= 128 ? 2 : 1;
+  return D <= (qb == 2 ? 48 : 64) ? 3 : D <= 128 ? 2 : 1;
+}
 template <typename T, int QB, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attention_e4m3_split_kernel(Args a) {
+__global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void attention_e4m3_split_kernel(Args a) {
   constexpr int PARTS = parts_of<T>(), TR = 16 * QB, RS = D + 4;
   __shared__ __attribute__((aligned(16))) float lds[split_lds_floats<QB, NW>()];
   float* s_m = lds + NW * TR * RS;
@@ -438,7 +447,7 @@ struct StagedSizes {
 };
 
 template <int RT, int P>
-__global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
+__global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
   typedef StagedSizes<RT, P> Z;
   constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DV = D / 32;
   constexpr int PIECES = KT * D / 1024;                          // loads of 1 KB of a stage's keys, and of its values
@@ -573,7 +582,7 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
     for (int j = 0; j < DK / 2; ++j) kc[j] = *(const uint4v*)(stage + k_at + j * 512);
     const float ks = power_of_byte(scales[0]);
     const float own_scale = power_of_byte(min((unsigned)scales[16], 254u));      // (finite: times a probability of zero it is zero)
-    if (h == 0) own_scales[col] = own_scale;
+    own_scales[col] = own_scale;      // (both halves the same)
     const unsigned there = there_next;
     there_next = fetch(tile + 1, slot ^ 1);
     const int kb0 = tile * KT + ph * 32;
@@ -601,8 +610,7 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : NEG_INF;
-      // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not keep
-      // out of the product: they become zeros, and the rows that do see them become no numbers.
+      // (codes that are not numbers: as in add_step)
       bool strange = false;
 #pragma unroll
       for (int block = 0; block < 2; ++block)
@@ -614,9 +622,12 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
       if (__any(strange)) {
 #pragma unroll
         for (int block = 0; block < 2; ++block) {
-          bf16x8 seen;
+          bf16x8 up, down;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) seen[i] = sees(block * 8 + i) ? (bf16_t)1.f : (bf16_t)0.f;
+          for (int i = 0; i < 8; ++i) {
+            up[i] = sees(block * 8 + i) ? (bf16_t)LARGE : (bf16_t)0.f;
+            down[i] = -up[i];
+          }
 #pragma unroll
           for (int group = 0; group < D / 64; ++group)
 #pragma unroll
@@ -625,16 +636,11 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
 #pragma unroll
               for (int x = 0; x < 8; ++x) {
                 const bool nan = ((vc[block][group][x >> 2][i] >> (8 * (x & 3))) & 0x7fu) == 0x7fu;
-                bad[x] = nan ? (bf16_t)1.f : (bf16_t)0.f;
+                bad[x] = nan ? (bf16_t)LARGE : (bf16_t)0.f;
                 if (nan) vc[block][group][x >> 2][i] &= ~(0xffu << (8 * (x & 3)));
               }
-              floatx16 hits;
-#pragma unroll
-              for (int x = 0; x < 16; ++x) hits[x] = 0.f;
-              hits = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bad, seen, hits, 0, 0, 0);
-#pragma unroll
-              for (int x = 0; x < 16; ++x)
-                if (hits[x] > 0.f) o[group * 2 + i][x] = __builtin_nanf("");
+              o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bad, up, o[group * 2 + i], 0, 0, 0);
+              o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bad, down, o[group * 2 + i], 0, 0, 0);
             }
         }
       }
@@ -678,13 +684,18 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
   __syncthreads();
   l += __shfl_xor(l, 32, WAVE);
 
+  // (the row's place worked out again: two registers less in the loop)
+  int again = row0 + col;
+  asm volatile("" : "+v"(again));
+  const bool has_row = again < total;
+  const int out_tok = has_row ? again / G : 0, out_head = kvh * G + (has_row ? again - out_tok * G : 0);
   // piece n of a row, four numbers: registers 4 (n % 4) .. + 3 of sum n / 4
   auto place = [&](int n) { return (n >> 3) * 64 + (((n & 3) >> 1) * 2 + ((n >> 2) & 1)) * 16 + (n & 1) * 8 + h * 4; };
   auto piece = [&](int n) { return floatx4{o[n >> 2][4 * (n & 3)], o[n >> 2][4 * (n & 3) + 1], o[n >> 2][4 * (n & 3) + 2], o[n >> 2][4 * (n & 3) + 3]}; };
   if constexpr (P == 1) {
-    if (valid)
+    if (has_row)
 #pragma unroll
-      for (int n = 0; n < DV * 4; ++n) write_output<bf16_t>(a, r0 + tok, head, place(n), piece(n), l);
+      for (int n = 0; n < DV * 4; ++n) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n), piece(n), l);
   } else {
     // group ph puts the pieces ph, ph + P, .. of its rows together; the others' it finds in LDS
     constexpr int SHARES = DV * 4 / P;
@@ -723,7 +734,7 @@ __global__ __launch_bounds__(64 * RT * P, 2) void attention_e4m3_staged_kernel(A
 #pragma unroll
       for (int p = 0; p < P; ++p)
         v += w[p] * (p == ph ? mine[n] : left[(((p * RT + rt) * SHARES + n) * (P - 1) + (ph > p ? ph - 1 : ph)) * 64 + lane]);
-      if (valid) write_output<bf16_t>(a, r0 + tok, head, place(n * P + ph), v, weight);
+      if (has_row) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n * P + ph), v, weight);
     }
   }
 }
@@ -788,21 +799,21 @@ static int key_splits(long blocks, int visible, int num_cus) {
 // for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
-// the picks lose 0.7 % (heads of 64) and 0.9 % (128) to the best of all (200 others: 1.3 %, 31 % at worst).  Up to 16 rows a
+// the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (250 others: 0.7 %, 15 % at worst).  Up to 16 rows a
 // tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
-// us, split / 2x4 / 2x2 / 4x1, heads of 128: 48 rows of 56 (request, kv head) pairs behind 6,732 keys 42 / 67 / 92 / 166; 126
-// of 92 behind 881 23.0 / 19.7 / 20.6 / 30.7; 504 of 44 behind 157 18 / 22 / 14 / 15.5; 7,990 of 8 and 1,598 keys 68 / 63 / 47 / 51;
-// 1,368 of 64 behind 309 61 / 70 / 47 / 44; 5,624 of 48 and 712 keys 163 / 188 / 113 / 104.
+// us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
+// of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
+// 1,304 of 40 behind 63 32 / 38 / 26 / 21.5; 6,624 of 48 behind 232 241 / 269 / 161 / 148.
 enum { FORM_SPLIT = 1, FORM_2x4, FORM_2x2, FORM_4x1 };
 #if STAGED
 static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
   if (most_rows <= 16) return FORM_SPLIT;
   struct Form { int rows, groups; float blocks_a_unit, start, step, more, least; };
-  constexpr Form forms[] = {{32, SPLIT_WAVES, 2.f, D == 64 ? 4.2f : 6.f, D == 64 ? .92f : 1.38f, D == 64 ? .6f : .67f, D == 64 ? 1.06f : .91f},
-                            {64, 4, 1.f, D == 64 ? 5.f : 8.2f, D == 64 ? .8f : 1.36f, D == 64 ? .65f : .42f, D == 64 ? 1.17f : .92f},
-                            {64, 2, D == 64 ? 3.f : 2.f, D == 64 ? 6.f : 8.2f, D == 64 ? .74f : .93f, D == 64 ? .73f : .67f, D == 64 ? .88f : .83f},
-                            {128, 1, D == 64 ? 3.f : 2.f, D == 64 ? 6.f : 10.5f, D == 64 ? .7f : .84f, D == 64 ? .89f : .67f, D == 64 ? .94f : .87f}};
-  constexpr float MERGE = D == 64 ? 3.9f : 1.8f;
+  constexpr Form forms[] = {{32, SPLIT_WAVES, D == 64 ? 3.f : 2.f, D == 64 ? 5.5f : 6.4f, D == 64 ? 1.14f : 1.18f, D == 64 ? .54f : .58f, D == 64 ? .79f : .92f},
+                            {64, 4, D == 64 ? 2.f : 1.f, D == 64 ? 6.f : 8.2f, D == 64 ? .85f : 1.18f, D == 64 ? .9f : .34f, D == 64 ? .83f : 1.f},
+                            {64, 2, D == 64 ? 4.f : 3.f, D == 64 ? 6.2f : 10.5f, D == 64 ? .75f : 1.06f, D == 64 ? .82f : .51f, .71f},
+                            {128, 1, D == 64 ? 4.f : 3.f, D == 64 ? 6.7f : 10.4f, D == 64 ? .63f : .97f, D == 64 ? .95f : .72f, D == 64 ? .71f : .8f}};
+  constexpr float MERGE = D == 64 ? 2.2f : 1.3f;
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 4; ++i) {

@@ -5,7 +5,7 @@ from llm_inference_lab_amd.kernels import build
 from test_kernel_registers import SIMD_REGISTERS, kernels, library
 
 
-@pytest.mark.parametrize("d,kernel,waves,least", [(64, "e4m3_staged", 3, 3), (128, "e4m3_staged", 2, 3), (64, "e4m3_split", 2, 3),
+@pytest.mark.parametrize("d,kernel,waves,least", [(64, "e4m3_staged", 4, 3), (128, "e4m3_staged", 2, 3), (64, "e4m3_split", 2, 3),
                                                   (128, "e4m3_split", 2, 3)])
 def test_waves_a_simd_holds(d, kernel, waves, least):
     taken = {name: v for name, v in kernels(library(lambda: build.e4m3_attention_library(d))).items() if kernel in name}
