@@ -11,20 +11,18 @@
 // The angles of the rotation, its products and the quantised numbers are taken in 64 bits: a position of 30,000 leaves
 // a float32 angle 2^-10 of a turn, and a number next to the border between two codes (one of 16 steps in an octave) goes
 // to the one that the formula says.  The vector unit takes float64 products at the float32 rate, and the pass over memory
-// bounds the kernel.
+// bounds the kernel.  8,192 rows of 28 heads of 128 over 4 (143 MB) take 37.5 us (3.8 TB/s; without the rotation 34): a row is a wave's
+// chain of loads, products and stores, its next heads asked for while some are turned.
 #include "common.h"
 
 constexpr int LOWEST_EXPONENT = -100;
 
-// v to 32 bits so that a rounding to fewer bits afterwards gives what one rounding of v gives: the last bit
-// is set where v lies between two float32 numbers (rounding to odd).
+// v to 32 bits so that a rounding to fewer bits afterwards gives what one rounding of v gives: cut off behind 24 bits, and the last
+// of them is set where anything was cut (rounding to odd).  What is finite stays finite.
 __device__ __forceinline__ float to_odd(double v) {
-  const float f = (float)v;
-  const double back = (double)f;
-  if (back == v || !(fabs(v) < __builtin_huge_val())) return f;
-  unsigned bits = __float_as_uint(f);
-  if (fabs(back) > fabs(v)) --bits;      // towards zero ...
-  return __uint_as_float(bits | 1u);     // ... and odd
+  const unsigned low = (unsigned)__double2loint(v), cut = low & 0x1fffffffu;
+  const float f = (float)__hiloint2double(__double2hiint(v), (int)((low ^ cut) | (cut ? 0x20000000u : 0u)));
+  return fabsf(f) == __builtin_huge_valf() && fabs(v) < __builtin_huge_val() ? copysignf(3.40282347e38f, f) : f;
 }
 
 // The byte of the scale for the largest magnitude `most` (finite, rounded to odd: no even number is crossed)
@@ -58,6 +56,34 @@ __device__ __forceinline__ size_t value_index(int k, int i, int d) {
          ((((k & 15) >> 2) * 16 + (i & 15)) * wide + ((i >> 4) & 3)) * 4 + (k & 3);
 }
 
+// Sine and cosine of an angle up to 2^31, to 2^-53: the nearest whole number k of quarter turns is taken off in two parts of pi / 2 (the
+// first product is exact inside the fma), Taylor's sums of the rest, |r| <= pi / 4, to r^15 and r^16 (what is left out:
+// r^17 / 17! < 5e-17), and k % 4 says which is which.
+__device__ __forceinline__ void sine_cosine(double angle, double* sine, double* cosine) {
+  const double k = rint(angle * 0.63661977236758134308);
+  const double r = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), x = r * r;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+  s = fma(s, x, 1.0 / 6227020800.0);
+  c = fma(c, x, -1.0 / 87178291200.0);
+  s = fma(s, x, -1.0 / 39916800.0);
+  c = fma(c, x, 1.0 / 479001600.0);
+  s = fma(s, x, 1.0 / 362880.0);
+  c = fma(c, x, -1.0 / 3628800.0);
+  s = fma(s, x, -1.0 / 5040.0);
+  c = fma(c, x, 1.0 / 40320.0);
+  s = fma(s, x, 1.0 / 120.0);
+  c = fma(c, x, -1.0 / 720.0);
+  s = fma(s, x, -1.0 / 6.0);
+  c = fma(c, x, 1.0 / 24.0);
+  c = fma(c, x, -0.5);
+  s = fma(s * x, r, r);
+  c = fma(c, x, 1.0);
+  const unsigned quarter = (unsigned)(long)k;
+  const double a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+  *sine = quarter & 2 ? -a : a;
+  *cosine = (quarter + 1) & 2 ? -b : b;
+}
+
 struct CacheArgs {
   const int* positions;
   const int* row_req;
@@ -80,26 +106,30 @@ __device__ __forceinline__ int page_of(const CacheArgs& a, int r, int* off) {
 }
 
 // N numbers of a row from an address that is aligned for it (WIDE) or not
+template <typename T, int N>
+struct Numbers {
+  typedef T vec __attribute__((ext_vector_type(N)));
+};
 template <typename T, int N, bool WIDE>
-__device__ __forceinline__ void load_numbers(const T* src, float (&x)[N]) {
-  if constexpr (WIDE) {
-    typedef T vec __attribute__((ext_vector_type(N)));
-    const vec v = *(const vec*)src;
+__device__ __forceinline__ typename Numbers<T, N>::vec load_numbers(const T* src) {
+  typedef typename Numbers<T, N>::vec vec;
+  if constexpr (WIDE) return *(const vec*)src;
+  vec v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_float((T)v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_float(src[i]);
-  }
+  for (int i = 0; i < N; ++i) v[i] = src[i];
+  return v;
 }
-template <typename T, int N, bool WIDE>
+// PAST: written past the caches (whole lines only: of half lines each would go to memory by itself)
+template <typename T, int N, bool WIDE, bool PAST = false>
 __device__ __forceinline__ void store_numbers(T* dst, const float (&x)[N]) {
   if constexpr (WIDE) {
-    typedef T vec __attribute__((ext_vector_type(N)));
-    vec v;
+    typename Numbers<T, N>::vec v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = from_float<T>(x[i]);
-    *(vec*)dst = v;
+    if constexpr (PAST)
+      __builtin_nontemporal_store(v, (decltype(v)*)dst);
+    else
+      *(decltype(v)*)dst = v;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) dst[i] = from_float<T>(x[i]);
@@ -120,33 +150,46 @@ __device__ __forceinline__ unsigned four_codes(const float (&x)[4], float inv) {
          (unsigned)to_code(x[3], inv) << 24;
 }
 
-// ROWS rows a block, WAVES waves a row.  A lane has four pairs of a head (channels 4 s .. 4 s + 3 and those half a head
-// further), so a wave of 64 has several heads at a time, whatever the head size.  Every lane takes the sine and cosine
-// of one pair of its row (of two above heads of 128) and they are shared through LDS.  With 16 rows a block (many rows: what the
-// block stores fills whole blocks of 16 keys on one die's L2) the values' codes meet in LDS: where four rows are the
-// four keys of a word of the pages, the word is stored, and else its bytes.
+// ROWS rows a block of WAVES waves, as many for every row.  A lane has four pairs of a head (channels 4 s .. 4 s + 3 and
+// those half a head further), so a wave of 64 has several heads at a time, whatever the head size.  Every lane takes the sine and
+// cosine of one pair of its row (of two above heads of 128) and they are shared through LDS.  Where a block has several
+// rows the values' codes meet in LDS: where four rows are the four keys of a word of the pages, the word is stored, and else
+// its bytes.
 template <typename T, int ROWS, int WAVES, bool WIDE>
-__global__ __launch_bounds__(64 * ROWS * WAVES) void rope_kv_write_e4m3_kernel(const T* qkv, size_t row_stride, const float* inv_freq,
-                                                                                 T* q_out, size_t q_stride, int rows, CacheArgs a) {
-  __shared__ double s_turn[ROWS * WAVES][256];      // [wave][d / 2 cosines, d / 2 sines]
+__global__ __launch_bounds__(64 * WAVES) void rope_kv_write_e4m3_kernel(const T* qkv, size_t row_stride, const float* inv_freq,
+                                                                          T* q_out, size_t q_stride, int rows, CacheArgs a) {
+  static_assert(WAVES % ROWS == 0 && (ROWS == 1 || WAVES % 4 == 0), "as many waves for every row, four for a word of keys");
+  __shared__ double s_turn[WAVES][256];             // [wave][d / 2 cosines, d / 2 sines]
   __shared__ int s_page[ROWS], s_off[ROWS];
-  extern __shared__ unsigned char s_codes[];        // [ROWS][nkv * d] where ROWS = 16
+  extern __shared__ unsigned char s_codes[];        // [ROWS][nkv * d] where ROWS > 1
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slot = wave / WAVES, r = blockIdx.x * ROWS + slot;
+  constexpr int EACH = WAVES / ROWS;                // waves of a row
+  const int slot = wave / EACH, r = blockIdx.x * ROWS + slot;
   const int d = a.d, half = d >> 1, lanes = half >> 2, heads_at_once = 64 / lanes;
   const int here = lane / lanes, sub = lane - here * lanes, i0 = sub * 4;
+  const int heads = a.nq + 2 * a.nkv;
   const bool live = r < rows;
+  // (no branch around a load: where it ends the compiler would wait for all that is on its way; past the heads the last one is read)
+  typename Numbers<T, 4>::vec next_lo, next_hi;
+  auto fetch = [&](int first) {
+    const T* src = qkv + (size_t)min(r, rows - 1) * row_stride + (size_t)min(first + here, heads - 1) * d;
+    next_lo = load_numbers<T, 4, WIDE>(src + i0);
+    next_hi = load_numbers<T, 4, WIDE>(src + i0 + half);
+  };
+  const int step = EACH * heads_at_once;
+  int first = wave % EACH * heads_at_once;
+  fetch(first);
   int off = 0;
   const int page = live ? page_of(a, r, &off) : -1;
-  if (lane == 0 && wave % WAVES == 0) {
+  if (lane == 0 && ROWS > 1 && wave % EACH == 0) {
     s_page[slot] = page;
     s_off[slot] = off;
   }
   double* turn = s_turn[wave];
   if (inv_freq && live) {
     const double pos = (double)a.positions[r];
-    for (int i = lane; i < half; i += 64) sincos(pos * (double)inv_freq[i], &turn[half + i], &turn[i]);
+    for (int i = lane; i < half; i += 64) sine_cosine(pos * (double)inv_freq[i], &turn[half + i], &turn[i]);
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -157,21 +200,25 @@ __global__ __launch_bounds__(64 * ROWS * WAVES) void rope_kv_write_e4m3_kernel(c
     c[j] = inv_freq && live ? turn[i0 + j] : 1.0;      // (a lane past the heads: within the row of 256, not used)
     s[j] = inv_freq && live ? turn[half + i0 + j] : 0.0;
   }
-  const int heads = a.nq + 2 * a.nkv;
-  for (int first = (wave % WAVES) * heads_at_once; live && first < heads; first += WAVES * heads_at_once) {
+  for (; live && first < heads; first += step) {
     const int head = first + here;
     const bool in = here < heads_at_once && head < heads;
     const bool is_q = head < a.nq, is_v = head >= a.nq + a.nkv;
-    const T* src = qkv + (size_t)r * row_stride + (size_t)(in ? head : first) * d;
+    const auto raw_lo = next_lo, raw_hi = next_hi;
+    fetch(first + step);
     float lo[4], hi[4], most = 0.f;
-    load_numbers<T, 4, WIDE>(src + i0, lo);
-    load_numbers<T, 4, WIDE>(src + i0 + half, hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo[j] = to_float((T)raw_lo[j]);
+      hi[j] = to_float((T)raw_hi[j]);
+    }
     if (inv_freq && !is_v) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double x = (double)lo[j], y = (double)hi[j];
-        lo[j] = to_odd(x * c[j] - y * s[j]);
-        hi[j] = to_odd(y * c[j] + x * s[j]);
+        const double p = x * c[j] - y * s[j], q = y * c[j] + x * s[j];
+        lo[j] = sizeof(T) == 4 && is_q ? (float)p : to_odd(p);
+        hi[j] = sizeof(T) == 4 && is_q ? (float)q : to_odd(q);
       }
     }
     if (in && is_q) {
@@ -201,7 +248,7 @@ __global__ __launch_bounds__(64 * ROWS * WAVES) void rope_kv_write_e4m3_kernel(c
     if (!is_v) {
       *(unsigned*)(a.k + at * d + key_index(off, i0, d)) = cl;
       *(unsigned*)(a.k + at * d + key_index(off, i0 + half, d)) = ch;
-    } else if constexpr (ROWS == 16) {
+    } else if constexpr (ROWS > 1) {
       unsigned char* dst = s_codes + ((size_t)slot * a.nkv + kvh) * d + i0;
       *(unsigned*)dst = cl;
       *(unsigned*)(dst + half) = ch;
@@ -213,20 +260,19 @@ __global__ __launch_bounds__(64 * ROWS * WAVES) void rope_kv_write_e4m3_kernel(c
       }
     }
   }
-  if constexpr (ROWS == 16) {
-    static_assert(WAVES == 1, "a wave a row");
+  if constexpr (ROWS > 1) {
     __syncthreads();
     const int width = a.nkv * d;
     // lane j: whether rows j .. j + 3 are the four keys of a word
-    const int j = lane & 15, jp = s_page[j], jo = s_off[j];
-    bool leads = lane < 13 && jp >= 0 && (jo & 3) == 0;
+    const int j = lane & (ROWS - 1), jp = s_page[j], jo = s_off[j];
+    bool leads = lane < ROWS - 3 && jp >= 0 && (jo & 3) == 0;
 #pragma unroll
-    for (int t = 1; t < 4; ++t) leads = leads && s_page[min(j + t, 15)] == jp && s_off[min(j + t, 15)] == jo + t;
+    for (int t = 1; t < 4; ++t) leads = leads && s_page[min(j + t, ROWS - 1)] == jp && s_off[min(j + t, ROWS - 1)] == jo + t;
     const unsigned leaders = (unsigned)__ballot(leads);
     // four waves a word of keys
     unsigned left = leaders;
     for (int n = 0; left; ++n, left &= left - 1) {
-      if (n != wave >> 2) continue;
+      if (n % (WAVES / 4) != wave >> 2) continue;
       const int row = __ffs(left) - 1;
       const int to_page = s_page[row], to_off = s_off[row];
       for (int n2 = (wave & 3) * 64 + lane; n2 < width; n2 += 256) {
@@ -242,98 +288,121 @@ __global__ __launch_bounds__(64 * ROWS * WAVES) void rope_kv_write_e4m3_kernel(c
     }
     const unsigned covered = leaders | leaders << 1 | leaders << 2 | leaders << 3;
     if (!(covered >> slot & 1) && page >= 0)
-      for (int n = lane; n < width; n += 64) {
+      for (int n = wave % EACH * 64 + lane; n < width; n += EACH * 64) {
         const int kvh = n / d, i = n - kvh * d;
         a.v[((size_t)page * a.nkv + kvh) * a.page_size * d + value_index(off, i, d)] = s_codes[(size_t)slot * width + n];
       }
   }
 }
 
-// ROWS rows a wave.  A lane takes 16 numbers of a key (16 consecutive bytes of the page) and writes them one after
-// the other; of values the up to four 16-wide blocks' words of a number, each with the codes of four keys, of which a row
-// takes one: all four where the wave's rows are the four keys of a word.
+// ROWS rows a wave, 1,024 of their numbers at a time, keys and then values.  What is read and what is written both are whole lines:
+// the codes are fetched 16 bytes a lane in the page's order (of four rows that are the four keys of a word: four
+// neighbouring lanes have the four keys' same sixteen, 64 consecutive bytes; of values 256 bytes a group), meet in LDS row by row, and
+// go out 16 bytes a lane in the rows' order, past the caches where there are many: 32,768 positions of 8 heads of 128, 67 MB read and
+// 134 written, 37.9 us (5.3 TB/s; through the caches 58, so too by half lines that the L2 puts together).  A word of values holds four keys of one number; four lanes turn four such words into four numbers of one key.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void read_kv_e4m3_kernel(T* k_out, T* v_out, int rows, CacheArgs a) {
   typedef unsigned uint4v __attribute__((ext_vector_type(4)));
-  const int lane = threadIdx.x & 63;
-  const int r0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * ROWS;
+  constexpr int COLUMNS = 1024, EACH = 16 / sizeof(T);      // numbers a store
+  __shared__ __attribute__((aligned(16))) unsigned char s_codes[4][ROWS][COLUMNS + 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = (blockIdx.x * 4 + wave) * ROWS;
   if (r0 >= rows) return;
-  const int d = a.d, sixteens = d >> 4, groups = (sixteens + 3) >> 2, width = a.nkv * d, n_rows = min(ROWS, rows - r0);
+  const int d = a.d, sixteens = d >> 4, groups = (sixteens + 3) >> 2, width = a.nkv * d;
+  const int n_rows = min(ROWS, rows - r0), mine = lane & (ROWS - 1);
+  // (where a row has no page, page 0 is read and zeros are written; a cache without pages is not read)
+  int my_off = 0;
+  const int my_page = mine < n_rows ? page_of(a, r0 + mine, &my_off) : -1;
   int page[ROWS], off[ROWS];
   bool word = ROWS == 4 && n_rows == 4;
 #pragma unroll
   for (int t = 0; t < ROWS; ++t) {
-    page[t] = t < n_rows ? page_of(a, r0 + t, &off[t]) : -1;
-    if (t >= n_rows) off[t] = 0;
+    page[t] = __builtin_amdgcn_readlane(my_page, t);
+    off[t] = __builtin_amdgcn_readlane(my_off, t);
     word = word && page[t] == page[0] && off[t] == (off[0] & ~3) + t;
   }
-  word = word && page[0] >= 0;
-  // keys
-  for (int n = lane; n < a.nkv * sixteens; n += 64) {
-    const int kvh = n / sixteens, six = n - kvh * sixteens;
-    uint4v codes[ROWS];
-    float size[ROWS];
+  const bool any = a.pages > 0;
+  unsigned char(*codes)[COLUMNS + 16] = s_codes[wave];
+  auto meet = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // columns col0 .. col0 + count - 1 of the rows, from LDS
+  auto write = [&](T* out, int col0, int count, int of_values) {
+    meet();
+    for (int c = lane * EACH; c < count; c += 64 * EACH) {
+      const int kvh = (col0 + c) / d;
+      unsigned byte[ROWS];
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-      const size_t at = ((size_t)max(page[t], 0) * a.nkv + kvh) * a.page_size;
-      codes[t] = a.pages > 0 ? *(const uint4v*)(a.k + at * d + key_index(off[t], six * 16, d)) : uint4v{0, 0, 0, 0};
-      size[t] = a.pages > 0 ? power_of_byte(a.scale[2 * at + off[t]]) : 0.f;
-    }
+      for (int t = 0; t < ROWS; ++t)
+        byte[t] = any ? a.scale[(((size_t)max(page[t], 0) * a.nkv + kvh) * 2 + of_values) * a.page_size + off[t]] : 0;
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-      if (t >= n_rows) break;
-      T* dst = k_out + (size_t)(r0 + t) * width + n * 16;
+      for (int t = 0; t < ROWS; ++t) {
+        if (t >= n_rows) break;
+        float x[EACH];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) decode_four(codes[t][2 * h + j], size[t], page[t] >= 0, x + 4 * j);
-        store_numbers<T, 8, true>(dst + 8 * h, x);
+        for (int i = 0; i < EACH; i += 4) decode_four(*(const unsigned*)&codes[t][c + i], power_of_byte(byte[t]), page[t] >= 0, x + i);
+        store_numbers<T, EACH, true, ROWS == 4>(out + (size_t)(r0 + t) * width + col0 + c, x);
       }
     }
+    meet();
+  };
+  for (int six0 = 0; six0 < a.nkv * sixteens; six0 += COLUMNS / 16) {
+    const int count = min(COLUMNS / 16, a.nkv * sixteens - six0);
+    const unsigned char* from = a.k + (size_t)max(my_page, 0) * a.nkv * a.page_size * d;
+#pragma unroll
+    for (int i = 0; i < COLUMNS / 16 * ROWS / 64; ++i) {
+      const int n = (i * 64 + lane) / ROWS, kvh = (six0 + n) / sixteens, six = six0 + n - kvh * sixteens;
+      if (n < count && any)
+        *(uint4v*)&codes[mine][n * 16] = *(const uint4v*)(from + (size_t)kvh * a.page_size * d + key_index(my_off, six * 16, d));
+    }
+    write(k_out, six0 * 16, count * 16, 0);
   }
-  // values: a lane has four neighbouring numbers of up to four 16-wide blocks, 64 consecutive bytes of the page
-  for (int n = lane; n < a.nkv * groups * 4; n += 64) {
-    const int kvh = n / (groups * 4), m = n - kvh * groups * 4, group = m >> 2, c = (m & 3) * 4;
-    const int wide = min(4, sixteens - 4 * group);
-    unsigned codes[ROWS][4][4];      // [row][number][block of the group]
-    float size[ROWS];
+  for (int g0 = 0; g0 < a.nkv * groups; g0 += COLUMNS / 64) {
+    const int count = min(COLUMNS / 64, a.nkv * groups - g0);
+    auto column = [&](int group) { return group / groups * d + group % groups * 64; };
+    const int col0 = column(g0), end = g0 + count < a.nkv * groups ? column(g0 + count) : width;
+    // a unit: number c of up to four 16-wide blocks
+    for (int u = lane; u < count * 16; u += 64) {
+      const int kvh = (g0 + (u >> 4)) / groups, g = g0 + (u >> 4) - kvh * groups, c = u & 15, wide = min(4, sixteens - 4 * g);
+      unsigned char* to = &codes[0][kvh * d + g * 64 - col0];
+      auto words = [&](int t, unsigned (&w)[4]) {
+        const unsigned char* at = a.v + ((size_t)max(page[t], 0) * a.nkv + kvh) * a.page_size * d;
+        const unsigned* src = (const unsigned*)(at + (value_index(off[t], g * 64 + c, d) & ~(size_t)3));
+        if (wide == 4) {
+          const uint4v x = *(const uint4v*)src;
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-      const size_t at = ((size_t)max(page[t], 0) * a.nkv + kvh) * a.page_size;
-      size[t] = a.pages > 0 ? power_of_byte(a.scale[2 * at + a.page_size + off[t]]) : 0.f;
-      const unsigned* src = (const unsigned*)(a.v + at * d + (value_index(off[t], group * 64 + c, d) & ~(size_t)3));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (word && t > 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) codes[t][i][j] = codes[0][i][j];
-        } else if (a.pages <= 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) codes[t][i][j] = 0;
-        } else if (wide == 4) {
-          const uint4v w = *(const uint4v*)(src + 4 * i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) codes[t][i][j] = w[j];
+          for (int b = 0; b < 4; ++b) w[b] = x[b];
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) codes[t][i][j] = src[i * wide + min(j, wide - 1)];
+          for (int b = 0; b < 4; ++b) w[b] = src[min(b, wide - 1)];
+        }
+      };
+      if (!any) continue;
+      unsigned w[4];
+      if (word) {
+        words(0, w);
+        const unsigned pick = 0x0400u + 0x0101u * (lane & 3);      // byte (lane % 4) of two words
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int v = (int)w[b];
+          const unsigned x0 = __builtin_amdgcn_update_dpp(0, v, 0x00, 0xf, 0xf, true), x1 = __builtin_amdgcn_update_dpp(0, v, 0x55, 0xf, 0xf, true),
+                         x2 = __builtin_amdgcn_update_dpp(0, v, 0xaa, 0xf, 0xf, true), x3 = __builtin_amdgcn_update_dpp(0, v, 0xff, 0xf, 0xf, true);
+          const unsigned low = __builtin_amdgcn_perm(x1, x0, pick), high = __builtin_amdgcn_perm(x3, x2, pick);
+          if (b < wide) *(unsigned*)(to + (size_t)mine * (COLUMNS + 16) + b * 16 + (c & ~3)) = __builtin_amdgcn_perm(high, low, 0x05040100u);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) {
+          words(t, w);
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (b < wide) to[(size_t)t * (COLUMNS + 16) + b * 16 + c] = (unsigned char)(w[b] >> (8 * (off[t] & 3)));
         }
       }
     }
-#pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-      if (t >= n_rows) break;
-      T* dst = v_out + (size_t)(r0 + t) * width + (size_t)kvh * d + group * 64 + c;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = page[t] >= 0 ? __builtin_amdgcn_cvt_f32_fp8(codes[t][i][j] >> (8 * (off[t] & 3)), 0) * size[t] : 0.f;
-        if (j < wide) store_numbers<T, 4, true>(dst + j * 16, x);
-      }
-    }
+    write(v_out, col0, end - col0, 1);
   }
 }
 
@@ -363,18 +432,23 @@ extern "C" int llmlab_rope_kv_write_e4m3(const void* qkv, int dtype, int rows, s
   const bool wide = (uintptr_t)qkv % (dtype == DT_BF16 ? 8 : 16) == 0 && (uintptr_t)q_out % (dtype == DT_BF16 ? 8 : 16) == 0 &&
                     row_stride % 4 == 0 && q_stride % 4 == 0;
   auto launch = [&](auto kernel, int rows_a_block, int waves, size_t lds, auto* x, auto* y) {
-    hipLaunchKernelGGL(kernel, dim3((rows + rows_a_block - 1) / rows_a_block), dim3(64 * rows_a_block * waves), lds, stream, x,
+    hipLaunchKernelGGL(kernel, dim3((rows + rows_a_block - 1) / rows_a_block), dim3(64 * waves), lds, stream, x,
                        row_stride, inv_freq, y, q_stride, rows, a);
   };
-  // Many rows: 16 a block where their values' codes fit beside the sines; few: as many waves a row as spread over the chip.
-  const size_t codes = (size_t)16 * nkv * d;
-  const bool many = rows >= 1024 && codes <= 31 * 1024;
+  // Many rows: eight a block, a wave each, where their values' codes fit beside the sines; few: four waves a row, so that a row's chain is
+  // short and the rows spread over the chip.  us, few / many: 14 heads of 64 over 2, 1,024 rows 6.1 / 7.4, 2,048 9.4 / 7.8, 8,192
+  // 26.8 / 17.4; 28 of 128 over 4 9.8 / 13.3, 14.5 / 14.1, 46.8 / 37.3; 64 of 128 over 8 14.0 / 23.2, 21.3 / 24.3, 78 / 77.  (Sixteen rows a block:
+  // 2,048 rows 19.2, 8,192 37.8; four: 13.8 and 40.1; two waves a row 13.2 and 45.8; all waves of a block over its rows one
+  // after the other 20.8 and 45.4.)
+  constexpr int MANY = 8;
+  const size_t codes = (size_t)MANY * nkv * d;
+  const bool many = rows >= 2048 && codes <= 31 * 1024;
   auto pick = [&](auto t) {
     typedef decltype(t) T;
     const T* x = (const T*)qkv;
     T* y = (T*)q_out;
     if (!wide) launch(rope_kv_write_e4m3_kernel<T, 1, 4, false>, 1, 4, 0, x, y);
-    else if (many) launch(rope_kv_write_e4m3_kernel<T, 16, 1, true>, 16, 1, codes, x, y);
+    else if (many) launch(rope_kv_write_e4m3_kernel<T, MANY, MANY, true>, MANY, MANY, codes, x, y);
     else launch(rope_kv_write_e4m3_kernel<T, 1, 4, true>, 1, 4, 0, x, y);
   };
   if (dtype == DT_BF16) pick(bf16_t());
@@ -393,9 +467,11 @@ extern "C" int llmlab_read_kv_e4m3(const void* k, const void* v, const void* sca
   if (rc) return rc;
   if (rows == 0) return 0;
   LLMLAB_REQUIRE((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "read_kv_e4m3: the outputs are not aligned to 16 bytes");
+  // Four rows a wave once the rows fill the chip so (us, four / one, 8 heads of 128: 2,048 rows in order 10.8 / 8.5, 8,192 14.8 / 14.2, 16,384
+  // 19.1 / 31.2; in any order 18.7 / 9.7, 23.7 / 19.1, 33.4 / 38.2).
   auto pick = [&](auto t) {
     typedef decltype(t) T;
-    if (rows >= 4096)
+    if (rows > 8192)
       hipLaunchKernelGGL((read_kv_e4m3_kernel<T, 4>), dim3((rows + 15) / 16), dim3(256), 0, stream, (T*)k_out, (T*)v_out, rows, a);
     else
       hipLaunchKernelGGL((read_kv_e4m3_kernel<T, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, (T*)k_out, (T*)v_out, rows, a);
