@@ -11,7 +11,9 @@
 // registers: a key's scale goes in with the conversion (one instruction makes two numbers and multiplies them), a value's
 // into its probability, in float32 behind the sum of the probabilities.  The numbers of a key are taken in the order in
 // which a lane's 16 bytes hold them (lane group g of a piece of 64: numbers 16 g .. 16 g + 15, the first eight in one
-// product and the others in the next), and the queries alike.  Scores, maxima, exponentials and sums are float32.
+// product and the others in the next), and the queries alike.  Scores, maxima, exponentials and sums are float32.  A probability
+// times its value's scale is rounded once, to the bfloat16 that the instruction takes (half a step, 2^-9 of itself: outputs 0.0022 off 64
+// bits, 0.0017 of it their own rounding).
 //
 // float32 queries are taken as three bfloat16 parts (24 bits: nothing is lost), probabilities too, each part a
 // product of its own; the keys' and values' numbers are exact.
@@ -158,7 +160,7 @@ __device__ __forceinline__ void load_rows(const Args& a, Rows<QB, PARTS>& r, int
 
 // One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  The running
 // maximum is kept in the units of the exponent and is raised only when a score exceeds it by more than LAZY_MAX: until then p may
-// be as large as 2^8, which float32 sums and bfloat16 probabilities hold without loss, and rescaling the sums is rare.
+// be as large as 2^8, which changes no rounding (bfloat16 has float32's exponents), and rescaling the sums is rare.
 template <bool MASKED, int QB, int PARTS>
 __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step& f, int kb, int g) {
   floatx4 s[2][QB];
@@ -267,7 +269,10 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 
 // Few rows a request: NW waves share a tile of 16 QB rows (a row: a token and a head of the group that shares a kv head) and
 // split the block's keys in steps of 32; their sums meet in LDS.  The keys of a tile are split over a.splits blocks as
-// well, whose sums a kernel of its own puts together.  Bound by the reading of the codes.
+// well, whose sums a kernel of its own puts together.  Bound by the reading of the codes where a request brings a token or a few: 64 requests
+// of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 41 and 5.5 of the merge; 32 of
+// 5 tokens of 40 heads over 8 at 2,500 (124 MB) 30.  float32 rows by their products, three a part: 7 of 61 tokens of 16 heads over 2 through a
+// window of 1,000 22 us.
 template <int QB, int NW>
 constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
 
@@ -416,6 +421,13 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 //     a lane holds of S^T; product i of a group of 64 numbers takes its 16-wide blocks i and 2 + i, as 8 bytes a lane
 //     hold blocks 0 and 1 (lanes 0 .. 15 of a half) or 2 and 3.
 // Every wave brings the scales of its group's keys itself, and makes float32 numbers of the values' ones in LDS.
+//
+// What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
+// instructions (512 clocks of a SIMD) and some 170 others (680 and more), 64 of them conversions; three portions of 1,000 tokens behind
+// 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 161 to 172 us (0.75 PFLOP/s), with half of the clocks in vector and a quarter in matrix
+// instructions, and a fifth of the units idle in the last round of blocks.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
+// loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
+// 2^-16 of the sum of sizes), so not used.
 #define STAGED (HEAD_DIM == 64 || HEAD_DIM == 128)
 #if STAGED
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;

@@ -1251,7 +1251,7 @@ class HipOps:
         table does not have are not seen, and a row that sees none gives zeros.  ``q`` and ``out [rows, heads * d]`` are
         both bfloat16 or both float32 (products in 24 bits); scores, softmax and sums are float32.  ``max_q_len`` and
         ``max_ctx_len`` are the longest portion and context among the requests.  Rows behind the last request keep what they
-        hold."""
+        hold.  Long contexts of few requests use the kernel set's workspace: calls of one kernel set go to one stream at a time."""
         self.prepare_attention_e4m3(q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
                                     q_start, start_pos, window, scale, out).launch(n_reqs, max_q_len, max_ctx_len)
 
