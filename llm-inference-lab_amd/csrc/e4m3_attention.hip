@@ -270,7 +270,7 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 // Few rows a request: NW waves share a tile of 16 QB rows (a row: a token and a head of the group that shares a kv head) and
 // split the block's keys in steps of 32; their sums meet in LDS.  The keys of a tile are split over a.splits blocks as
 // well, whose sums a kernel of its own puts together.  Bound by the reading of the codes where a request brings a token or a few: 64 requests
-// of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 41 and 5.5 of the merge; 32 of
+// of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 40 and 4.7 of the merge; 32 of
 // 5 tokens of 40 heads over 8 at 2,500 (124 MB) 30.  float32 rows by their products, three a part: 7 of 61 tokens of 16 heads over 2 through a
 // window of 1,000 22 us.
 template <int QB, int NW>
@@ -752,38 +752,51 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 }
 #endif  // STAGED
 
-// The splits of a row put together: a wave a (row, head), four numbers a lane.
+// The splits of a row put together: a wave a (row, head), four numbers a lane and, where a head leaves lanes over, several splits at a
+// time.  All of up to 8 splits a group of lanes are on their way while the factors are worked out (a lane a split).
 template <typename T>
 __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
+  constexpr int LANES = D / 4, GROUPS = 64 % LANES == 0 ? 64 / LANES : 1, AT_ONCE = 8;
   const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = at / a.nq;
   if (row < a.q_start[0] || row >= a.q_start[a.reqs] || row >= a.rows) return;
+  const int group = lane / LANES < GROUPS ? lane / LANES : 0, i = GROUPS > 1 ? lane % LANES * 4 : lane * 4;
   const float* ml = a.ml_part + (size_t)at * a.splits * 2;
-  float top = NEG_INF, l = 0.f;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[2 * s]);
-  top = full_wave_max(top);
-  const float* o = a.o_part + (size_t)at * a.splits * D;
+  const float* o = a.o_part + (size_t)at * a.splits * D + (i < D ? i : 0);
+  floatx4 x[AT_ONCE];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) x[j] = *(const floatx4*)(o + (size_t)min(s0 + j * GROUPS + group, a.splits - 1) * D);
+  };
+  fetch(0);
+  float m[2], w[2], f[2];      // (at most 128 splits)
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int s = lane + 64 * n;
+    m[n] = s < a.splits ? ml[2 * s] : NEG_INF;
+    w[n] = s < a.splits ? ml[2 * s + 1] : 0.f;
+  }
+  const float top = full_wave_max(fmaxf(m[0], m[1]));
+#pragma unroll
+  for (int n = 0; n < 2; ++n) f[n] = m[n] == NEG_INF ? 1.f : fast_exp2(m[n] - top);
+  const float l = full_wave_sum(f[0] * w[0] + f[1] * w[1]);
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  const int i = lane * 4;
-  for (int s0 = 0; s0 < a.splits; s0 += 4) {      // four splits' loads at a time
-    floatx4 x[4];
-    float m[4], w[4];
+  for (int s0 = 0; s0 < a.splits; s0 += AT_ONCE * GROUPS) {
+    if (s0 > 0) fetch(s0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int s = min(s0 + j, a.splits - 1);
-      m[j] = ml[2 * s];
-      w[j] = ml[2 * s + 1];
-      x[j] = *(const floatx4*)(o + (size_t)s * D + (i < D ? i : 0));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (s0 + j >= a.splits) continue;
-      const float f = m[j] == NEG_INF ? 1.f : fast_exp2(m[j] - top);
-      sum += f * x[j];
-      l += f * w[j];
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int s = s0 + j * GROUPS + group;
+      const float low = __shfl(f[0], s & 63, WAVE), high = __shfl(f[1], s & 63, WAVE);
+      if (s < a.splits) sum += (s < 64 ? low : high) * x[j];
     }
   }
-  if (i < D) write_output<T>(a, row, at - row * a.nq, i, sum, l);
+  if constexpr (GROUPS > 1) {
+#pragma unroll
+    for (int off = LANES; off < 64; off <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor(sum[j], off, WAVE);
+  }
+  if (GROUPS > 1 ? lane < LANES : i < D) write_output<T>(a, row, at - row * a.nq, i, sum, l);
 }
 
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
@@ -800,7 +813,7 @@ extern "C" void llmlab_debug_attention_e4m3(int splits, int form) {
 constexpr int SPLIT_WAVES = 4;
 // Key splits: two blocks a unit where the tiles alone leave units without one; none shorter than 8 steps of 32 keys, and none of
 // up to 32 steps, where the launch that puts the splits together costs what they gain (one to 16 requests of 28 heads of 128 over 4 at 700
-// to 1,000 keys 8.3 to 10.5 us of GPU in one launch, 8.5 to 10.2 in two, and the host 2.5 us less; at 1,500 12.1 and 9.2).
+// to 1,000 keys 7.9 to 10.3 us of GPU in one launch, 8.1 to 10.3 in two, and the host 2.8 us less; at 1,500 11.4 and 8.4).
 static int key_splits(long blocks, int visible, int num_cus) {
   const long steps = (visible + 31) / 32, most = (steps + 7) / 8;
   if (blocks >= num_cus || steps <= 32) return 1;
@@ -811,7 +824,7 @@ static int key_splits(long blocks, int visible, int num_cus) {
 // for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
-// the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (250 others: 0.7 %, 15 % at worst).  Up to 16 rows a
+// the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (850 others: 0.9 %, 32 % at worst, requests of very different lengths).  Up to 16 rows a
 // tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
 // us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
 // of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
