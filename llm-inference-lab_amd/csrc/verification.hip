@@ -67,10 +67,40 @@ __device__ __forceinline__ double weight(float z, float most, double rate) { ret
 
 __device__ __forceinline__ bool bounded(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
+// Sums over the wave by lane swaps and DPP, no trip through LDS: every lane has the whole (wave_sum64), or what lies up to it
+// (running_sum).  All 64 lanes are active.
+__device__ __forceinline__ double of_halves(unsigned high, unsigned low) { return __hiloint2double((int)high, (int)low); }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double moved(double v) {      // zero where nothing comes from
+  return of_halves(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, ROWS == 0xf),
+                   __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, ROWS == 0xf));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
-  return v;
+  {
+    const auto h = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+    const auto l = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+    v = of_halves(h[0], l[0]) + of_halves(h[1], l[1]);
+  }
+  {
+    const auto h = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+    const auto l = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+    v = of_halves(h[0], l[0]) + of_halves(h[1], l[1]);
+  }
+  v += moved<0x128>(v);      // row_ror:8
+  v += moved<0x124>(v);      // row_ror:4
+  v += moved<0x4E>(v);       // quad_perm 2, 3, 0, 1
+  return v + moved<0xB1>(v); // quad_perm 1, 0, 3, 2
+}
+__device__ __forceinline__ double running_sum(double v) {
+  v += moved<0x111>(v);      // row_shr:1
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xa>(v); // row_bcast:15 into rows 1 and 3
+  return v + moved<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ double lane_value64(double v, int lane) {      // (the same lane for the whole wave)
+  return of_halves(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
 __device__ __forceinline__ int wave_min(int v) {
 #pragma unroll
@@ -180,7 +210,7 @@ __device__ __forceinline__ RowSum whole_row(const VerifyArgs& a, int row, double
   }
   RowSum r;
   r.most = full_wave_max(most);
-  r.best = wave_min(most == r.most ? best : NONE);
+  r.best = rate == 0.0 ? wave_min(most == r.most ? best : NONE) : NONE;      // (asked for where greedy)
   r.sum = wave_sum64(bounded(most) && bounded(r.most) ? sum * weight(most, r.most, rate) : 0.0);
   return r;
 }
@@ -211,25 +241,14 @@ __device__ __forceinline__ void chunk_weights(const VerifyArgs& a, const Source&
   }
 }
 
-// The running sum over the wave's lanes, one number a lane
-__device__ __forceinline__ double running_sum(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double x = __shfl_up(v, off, WAVE);
-    if (lane >= off) v += x;
-  }
-  return v;
-}
-
 // Of the chunks' masses (lane c of a round of 64 has chunk base + c), by one wave: the first positive one in which the running
 // sum reaches u times the whole (the last positive one where roundings keep the sum short of it), and what is left there.
 template <typename F>
 __device__ __forceinline__ int pick_chunk(int chunks, double u, F mass, double* left) {
   const int lane = threadIdx.x & 63;
   const double first = lane < chunks ? mass(lane) : 0.0;
-  double total = __shfl(running_sum(first), 63, WAVE);
-  for (int base = 64; base < chunks; base += 64) total += __shfl(running_sum(base + lane < chunks ? mass(base + lane) : 0.0), 63, WAVE);
+  double total = wave_sum64(first);
+  for (int base = 64; base < chunks; base += 64) total += wave_sum64(base + lane < chunks ? mass(base + lane) : 0.0);
   if (!(total > 0.0)) return -1;
   const double target = u * total;
   double run = 0.0;
@@ -242,10 +261,10 @@ __device__ __forceinline__ int pick_chunk(int chunks, double u, F mass, double* 
     const int at = use ? __ffsll(use) - 1 : positive ? 63 - __clzll(positive) : -1;
     if (at >= 0) {
       chunk = base + at;
-      *left = target - (__shfl(sum, at, WAVE) - __shfl(m, at, WAVE));
+      *left = target - (lane_value64(sum, at) - lane_value64(m, at));
     }
     if (use) break;
-    run = __shfl(sum, 63, WAVE);
+    run = lane_value64(sum, 63);
   }
   return chunk;
 }
