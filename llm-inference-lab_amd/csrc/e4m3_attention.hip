@@ -410,7 +410,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 }
 
 // ------------------------------------------------------------- many rows, codes staged in LDS
-// bfloat16 rows at heads of 64 and 128.  A block has RT tiles of 32 rows side by side, and P groups of waves that
+// bfloat16 rows at heads up to 128.  A block has RT tiles of 32 rows side by side, and P groups of waves that
 // take the staged keys in turn, 32 of every 32 P; the groups' sums meet in LDS at the end.  The codes come by direct loads
 // into LDS, in the cache's order, in two stages, one being multiplied while the other is on its way, one barrier a
 // stage, and become bfloat16 numbers behind the read from LDS: half the bytes there and on the way.  Products by
@@ -419,7 +419,9 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 //     16 (2 j + h) .. + 15 of its key, in two products, and the queries lie alike;
 //   O^T[d, row] = V^T . P^T: the keys of a block of 16 in the order {4 h .. + 3, 8 + 4 h .. + 3} for half h, which is what
 //     a lane holds of S^T; product i of a group of 64 numbers takes its 16-wide blocks i and 2 + i, as 8 bytes a lane
-//     hold blocks 0 and 1 (lanes 0 .. 15 of a half) or 2 and 3.
+//     hold blocks 0 and 1 (lanes 0 .. 15 of a half) or 2 and 3; a last group of fewer blocks alike, by words.
+// In LDS a block of 16 keys (or values) begins at a whole KB; where a head is no multiple of 64 the lanes past its end bring its last 16
+// bytes again, which nobody reads.
 // Every wave brings the scales of its group's keys itself, and makes float32 numbers of the values' ones in LDS.
 //
 // What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 // instructions, and a fifth of the units idle in the last round of blocks.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
 // loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
 // 2^-16 of the sum of sizes), so not used.
-#define STAGED (HEAD_DIM == 64 || HEAD_DIM == 128)
+#define STAGED (HEAD_DIM <= 128)
 #if STAGED
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
 
@@ -450,22 +452,26 @@ __device__ __forceinline__ int table_entry(const int* table, int at) {
   return v;
 }
 
+constexpr int PB = (D + 63) / 64, BLOCK = PB * 1024;             // loads of 1 KB, and bytes in LDS, of 16 keys
+constexpr int FULL = D / 64, REST = D / 16 % 4;                  // groups of four 16-wide blocks of a value, and blocks of the last one
+constexpr int REST_DV = (REST + 1) / 2, DV = 2 * FULL + REST_DV; // products of the last group, of all
+constexpr int GROUPS = FULL + (REST > 0);
+
 template <int RT, int P>
 struct StagedSizes {
   static constexpr int NW = RT * P, KT = 32 * P;
-  static constexpr int V_AT = KT * D, SCALES_AT = 2 * KT * D, STAGE = SCALES_AT + NW * 512;
-  static constexpr int STAGES = 2 * STAGE, SUMS = RT * (P - 1) * 32 * D * 4;
+  static constexpr int V_AT = KT / 16 * BLOCK, SCALES_AT = 2 * V_AT, STAGE = SCALES_AT + NW * 512;
+  static constexpr int STAGES = 2 * STAGE, SUMS = RT * (P - 1) * DV * 4096;
   static constexpr int LDS = (STAGES > SUMS ? STAGES : SUMS) + NW * 32 * 4 * 3;
 };
 
 template <int RT, int P>
-__global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
+__global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
   typedef StagedSizes<RT, P> Z;
-  constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DV = D / 32;
-  constexpr int PIECES = KT * D / 1024;                          // loads of 1 KB of a stage's keys, and of its values
+  constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DJ = (DK + 1) / 2;
+  constexpr int PIECES = KT / 16 * PB;                           // loads of 1 KB of a stage's keys, and of its values
   constexpr int EACH = PIECES * 2 / NW;                          // ... of a wave
   constexpr int HALF = EACH > 1 ? EACH / 2 : 1;                  // ... of keys, and of values (one: keys by even waves)
-  constexpr int PB = D / 64;                                     // pieces of a block of 16 keys
   constexpr int BLOCKS = HALF > PB ? HALF / PB : 1;              // blocks of 16 that a wave's pieces belong to
   static_assert(EACH * NW == PIECES * 2 && (EACH == 1 || EACH % 2 == 0), "whole loads a wave");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Z::LDS];
@@ -537,11 +543,12 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 #pragma unroll
       for (int i = 0; i < HALF / BLOCKS; ++i) {
         const unsigned to_piece = to + (piece0 + n * PB + i) * 1024;
+        const unsigned from = D % 64 == 0 ? lane * 16 : min(lane * 16, 16 * D - 16 - (piece0 % PB + i) * 1024);
         if constexpr (EACH > 1) {
-          load_1k(lane * 16, a.k + at + i * 1024, to_piece);
-          load_1k(lane * 16, a.v + at + i * 1024, to_piece + Z::V_AT);
+          load_1k(from, a.k + at + i * 1024, to_piece);
+          load_1k(from, a.v + at + i * 1024, to_piece + Z::V_AT);
         } else {
-          load_1k(lane * 16, (wave & 1 ? a.v : a.k) + at, wave & 1 ? to_piece + Z::V_AT : to_piece);
+          load_1k(from, (wave & 1 ? a.v : a.k) + at, wave & 1 ? to_piece + Z::V_AT : to_piece);
         }
       }
     }
@@ -555,18 +562,18 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
     return there;
   };
 
-  bf16x8 q[DK];
+  bf16x8 q[2 * DJ];
   {
     const bf16_t* qp = (const bf16_t*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
 #pragma unroll
-    for (int k = 0; k < DK; ++k) q[k] = *(const bf16x8*)(qp + ((k >> 1) * 2 + h) * 16 + (k & 1) * 8);
+    for (int k = 0; k < 2 * DJ; ++k) q[k] = *(const bf16x8*)(qp + min((k >> 1) * 2 + h, DK - 1) * 16 + (k & 1) * 8);
   }
   locate(tile_lo);
   // (waited for here, with the table: in the loop it would be waited for, with all that is on its way, in every step)
 #pragma unroll
-  for (int k = 0; k < DK; ++k) {
+  for (int k = 0; k < 2 * DJ; ++k) {
     const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-    q[k] = valid ? q[k] : zero;
+    q[k] = valid && (DK % 2 == 0 || (k >> 1) * 2 + h < DK) ? q[k] : zero;      // (a sixteen past the last: its keys' last one, times zero)
     asm volatile("" : "+v"(q[k]));
   }
   floatx16 o[DV];
@@ -577,7 +584,8 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
   float m = NEG_INF, l = 0.f;
   unsigned there_next = fetch(tile_lo, 0);
   float* const own_scales = own + wave * 32;
-  const int k_at = (ph * 2 + odd) * 16 * D + h * 256 + c * 16, v_at = Z::V_AT + ph * 32 * D + h * 256 + c * 16 + odd * 8;
+  const int k_at = (ph * 2 + odd) * BLOCK + h * 256 + c * 16, k_last = DK % 2 == 0 ? k_at : k_at - h * 256;
+  const int v_at = Z::V_AT + ph * 2 * BLOCK;
   for (int tile = tile_lo; tile <= tile_hi; ++tile) {
     // this tile's loads are in (the wave's own; behind the barrier, all), and the tile before is read by all
     __builtin_amdgcn_s_waitcnt(0x0070);
@@ -589,9 +597,9 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
     const int slot = (tile - tile_lo) & 1;
     const unsigned char* const stage = lds + slot * Z::STAGE;
     const unsigned char* const scales = stage + Z::SCALES_AT + wave * 512 + odd * 256 + c;
-    uint4v kc[DK / 2];
+    uint4v kc[DJ];
 #pragma unroll
-    for (int j = 0; j < DK / 2; ++j) kc[j] = *(const uint4v*)(stage + k_at + j * 512);
+    for (int j = 0; j < DJ; ++j) kc[j] = *(const uint4v*)(stage + (j + 1 < DJ ? k_at : k_last) + j * 512);
     const float ks = power_of_byte(scales[0]);
     const float own_scale = power_of_byte(min((unsigned)scales[16], 254u));      // (finite: times a probability of zero it is zero)
     own_scales[col] = own_scale;      // (both halves the same)
@@ -602,19 +610,28 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 #pragma unroll
     for (int x = 0; x < 16; ++x) s[x] = 0.f;
 #pragma unroll
-    for (int j = 0; j < DK / 2; ++j) {
+    for (int j = 0; j < DJ; ++j) {
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][0], kc[j][1], ks), q[2 * j], s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][2], kc[j][3], ks), q[2 * j + 1], s, 0, 0, 0);
     }
     // the values' codes travel while the maximum is found: [block of 16][group of 64][quad h or 2 + h], two blocks of 16 of d each
     typedef unsigned uint2v __attribute__((ext_vector_type(2)));
-    uint2v vc[2][D / 64][2];
+    uint2v vc[2][GROUPS][2];
 #pragma unroll
     for (int block = 0; block < 2; ++block)
 #pragma unroll
-      for (int group = 0; group < D / 64; ++group)
+      for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-        for (int two = 0; two < 2; ++two) vc[block][group][two] = *(const uint2v*)(stage + v_at + block * 16 * D + group * 1024 + two * 512);
+        for (int two = 0; two < 2; ++two) {
+          const int wide = group < FULL ? 4 : REST;
+          const unsigned char* at = stage + v_at + block * BLOCK + group * 1024 + (two * 32 + h * 16 + c) * 4 * wide;
+          if (wide == 4) {
+            vc[block][group][two] = *(const uint2v*)(at + odd * 8);
+          } else {
+            vc[block][group][two][0] = *(const unsigned*)(at + (wide == 1 ? 0 : odd * (wide == 3 ? 8 : 4)));
+            vc[block][group][two][1] = wide == 3 ? *(const unsigned*)(at + (odd ? 8 : 4)) : 0u;
+          }
+        }
     const bool masked = !(kb0 + 31 <= p_first && kb0 >= full_lo && there == 3);
     auto sees = [&](int i) {
       return (there >> (i >> 3) & 1) != 0 && (unsigned)(kb0 + 8 * (i >> 2) + (i & 3) + lane_key) <= span;
@@ -627,7 +644,7 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 #pragma unroll
       for (int block = 0; block < 2; ++block)
 #pragma unroll
-        for (int group = 0; group < D / 64; ++group)
+        for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
           for (int n = 0; n < 4; ++n)
             strange |= (((vc[block][group][n >> 1][n & 1] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
@@ -641,9 +658,9 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
             down[i] = -up[i];
           }
 #pragma unroll
-          for (int group = 0; group < D / 64; ++group)
+          for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < (group < FULL ? 2 : REST_DV); ++i) {
               bf16x8 bad;
 #pragma unroll
               for (int x = 0; x < 8; ++x) {
@@ -685,9 +702,9 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 #pragma unroll
       for (int i = 0; i < 8; ++i) pf[i] = (bf16_t)(p[i] * (i < 4 ? w0[i & 3] : w1[i & 3]));
 #pragma unroll
-      for (int group = 0; group < D / 64; ++group)
+      for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < (group < FULL ? 2 : REST_DV); ++i)
           o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(vc[block][group][0][i], vc[block][group][1][i], 1.f), pf,
                                                                      o[group * 2 + i], 0, 0, 0);
     }
@@ -702,12 +719,17 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
   const bool has_row = again < total;
   const int out_tok = has_row ? again / G : 0, out_head = kvh * G + (has_row ? again - out_tok * G : 0);
   // piece n of a row, four numbers: registers 4 (n % 4) .. + 3 of sum n / 4
-  auto place = [&](int n) { return (n >> 3) * 64 + (((n & 3) >> 1) * 2 + ((n >> 2) & 1)) * 16 + (n & 1) * 8 + h * 4; };
+  // (numbers past the head's end, of a last group of one or three 16-wide blocks: negative)
+  auto place = [&](int n) {
+    const int group = n >> 3, block = ((n & 3) >> 1) * (group < FULL ? 2 : REST_DV) + ((n >> 2) & 1);
+    return REST % 2 == 0 || group < FULL || block < REST ? group * 64 + block * 16 + (n & 1) * 8 + h * 4 : -1;
+  };
   auto piece = [&](int n) { return floatx4{o[n >> 2][4 * (n & 3)], o[n >> 2][4 * (n & 3) + 1], o[n >> 2][4 * (n & 3) + 2], o[n >> 2][4 * (n & 3) + 3]}; };
   if constexpr (P == 1) {
     if (has_row)
 #pragma unroll
-      for (int n = 0; n < DV * 4; ++n) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n), piece(n), l);
+      for (int n = 0; n < DV * 4; ++n)
+        if (place(n) >= 0) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n), piece(n), l);
   } else {
     // group ph puts the pieces ph, ph + P, .. of its rows together; the others' it finds in LDS
     constexpr int SHARES = DV * 4 / P;
@@ -746,7 +768,8 @@ __global__ __launch_bounds__(64 * RT * P, D == 64 ? 4 : P < 4 ? 3 : 2) void atte
 #pragma unroll
       for (int p = 0; p < P; ++p)
         v += w[p] * (p == ph ? mine[n] : left[(((p * RT + rt) * SHARES + n) * (P - 1) + (ph > p ? ph - 1 : ph)) * 64 + lane]);
-      if (has_row) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n * P + ph), v, weight);
+      const int to = place(n * P + ph);
+      if (has_row && to >= 0) write_output<bf16_t>(a, r0 + out_tok, out_head, to, v, weight);
     }
   }
 }
@@ -820,11 +843,12 @@ static int key_splits(long blocks, int visible, int num_cus) {
   return (int)std::max(1L, std::min(std::min(2L * num_cus / blocks, most), 128L));
 }
 
-// The form of a bfloat16 launch at heads of 64 and 128: the one whose time is the least by an estimate, rounds of blocks (`more`
+// The form of a bfloat16 launch at heads up to 128: the one whose time is the least by an estimate, rounds of blocks (`more`
 // for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
-// the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (850 others: 0.9 %, 32 % at worst, requests of very different lengths).  Up to 16 rows a
+// the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (850 others: 0.9 %, 32 % at worst, requests of very different lengths; 500 at heads of
+// 16 to 112, by the figures of 64 or 128, 0.9 %).  Up to 16 rows a
 // tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
 // us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
 // of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
@@ -834,11 +858,11 @@ enum { FORM_SPLIT = 1, FORM_2x4, FORM_2x2, FORM_4x1 };
 static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
   if (most_rows <= 16) return FORM_SPLIT;
   struct Form { int rows, groups; float blocks_a_unit, start, step, more, least; };
-  constexpr Form forms[] = {{32, SPLIT_WAVES, D == 64 ? 3.f : 2.f, D == 64 ? 5.5f : 6.4f, D == 64 ? 1.14f : 1.18f, D == 64 ? .54f : .58f, D == 64 ? .79f : .92f},
-                            {64, 4, D == 64 ? 2.f : 1.f, D == 64 ? 6.f : 8.2f, D == 64 ? .85f : 1.18f, D == 64 ? .9f : .34f, D == 64 ? .83f : 1.f},
-                            {64, 2, D == 64 ? 4.f : 3.f, D == 64 ? 6.2f : 10.5f, D == 64 ? .75f : 1.06f, D == 64 ? .82f : .51f, .71f},
-                            {128, 1, D == 64 ? 4.f : 3.f, D == 64 ? 6.7f : 10.4f, D == 64 ? .63f : .97f, D == 64 ? .95f : .72f, D == 64 ? .71f : .8f}};
-  constexpr float MERGE = D == 64 ? 2.2f : 1.3f;
+  constexpr Form forms[] = {{32, SPLIT_WAVES, D <= 64 ? 3.f : 2.f, D <= 64 ? 5.5f : 6.4f, D <= 64 ? 1.14f : 1.18f, D <= 64 ? .54f : .58f, D <= 64 ? .79f : .92f},
+                            {64, 4, D <= 64 ? 2.f : 1.f, D <= 64 ? 6.f : 8.2f, D <= 64 ? .85f : 1.18f, D <= 64 ? .9f : .34f, D <= 64 ? .83f : 1.f},
+                            {64, 2, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.2f : 10.5f, D <= 64 ? .75f : 1.06f, D <= 64 ? .82f : .51f, .71f},
+                            {128, 1, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.7f : 10.4f, D <= 64 ? .63f : .97f, D <= 64 ? .95f : .72f, D <= 64 ? .71f : .8f}};
+  constexpr float MERGE = D <= 64 ? 2.2f : 1.3f;
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 4; ++i) {
