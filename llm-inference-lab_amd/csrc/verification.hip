@@ -12,11 +12,11 @@
 // weights has a border every 1e-5 or so, and float32 sums taken in another order would cross one in every few hundred
 // draws.  What is summed is summed in one fixed order.
 //
-// Two launches: the rows in chunks (each leaves its maximum, its place and its sum of exponentials), then a block for every
-// chunk of every request's reached row, which finds that row from the chunks' sums, weighs its chunk, and is the one that
-// draws if it is the last of its request.  64 requests, 578 rows of 152,064 (351 MB): the first launch takes 68 us (5.2 TB/s; by a
-// polynomial of degree 12 with conversions 89), bound by its exponentials and the reading alike, the second 30: a chain of
-// small steps, 12 us for one request alone (first rows, sums, weights, the count of blocks, the chunk, the place in it).
+// Two launches: the rows in chunks (each leaves its maximum, its place and its sum of exponentials), then blocks for the
+// chunks of every request's reached row, which find that row from the chunks' sums and weigh their chunks; the last of a request
+// draws.  64 requests, 578 rows of 152,064 (351 MB): the first launch takes 65 us (5.4 TB/s; by a
+// polynomial of degree 12 with conversions 89), bound by its exponentials and the reading alike, the second 27: a chain of
+// small steps, 10 us for one request alone (first rows, sums, weights, the count of blocks, the chunk, the place in it).
 #include "common.h"
 
 constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH;
@@ -34,6 +34,7 @@ struct VerifyArgs {
   int* tokens;
   size_t stride, draft_stride;
   int n, rows, vocab, chunks;
+  int each;                  // chunks that a block of the second launch weighs
   // scratch
   double* sum;               // [rows + drafted, chunks]: sum of exp((z - chunk's maximum) / t)
   double* mass;              // [n, chunks]: what the chunk weighs in the draw
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(VerifyArgs a) {
   __shared__ int s_last, s_chunk, s_plain;
   __shared__ double s_sum[WAVES], s_left;
   __shared__ RowSum s_row[2 * AT_ONCE + 1];
-  const int chunk = blockIdx.x, b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int chunk = blockIdx.x * a.each, b = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r0 = a.row_start[b];
   int count = a.row_start[b + 1] - r0;
   const float t = a.temperature[b];
@@ -366,22 +367,28 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(VerifyArgs a) {
   }
   if (greedy || !sound) return;
 
-  // this chunk's weight
-  double w[EACH], mine = 0.0;
-  chunk_weights(a, d, chunk * CHUNK, w);
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) mine += w[j];
-  mine = wave_sum64(mine);
-  if (lane == 0) s_sum[wave] = mine;
-  __syncthreads();
+  // its chunks' weights
+  double w[EACH];
   double* mass = a.mass + (size_t)b * a.chunks;
+  for (int c = chunk; c < min(chunk + a.each, a.chunks); ++c) {
+    double mine = 0.0;
+    chunk_weights(a, d, c * CHUNK, w);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) mine += w[j];
+    mine = wave_sum64(mine);
+    __syncthreads();
+    if (lane == 0) s_sum[wave] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double total = 0.0;
+      for (int i = 0; i < WAVES; ++i) total += s_sum[i];
+      // (device scope: past this die's L2, and done before the count)
+      __hip_atomic_store(&mass[c], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
   if (threadIdx.x == 0) {
-    double total = 0.0;
-    for (int i = 0; i < WAVES; ++i) total += s_sum[i];
-    // (device scope: past this die's L2, and done before the count)
-    __hip_atomic_store(&mass[chunk], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);
-    s_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+    s_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   }
   __syncthreads();
   if (!s_last) return;
@@ -492,7 +499,7 @@ extern "C" int llmlab_verify_drafts(const float* logits, size_t stride, const fl
   LLMLAB_REQUIRE(scratch_bytes >= llmlab_verify_drafts_scratch(n, rows, vocab, draft != nullptr) && ((uintptr_t)scratch % 8) == 0,
                  "verify_drafts: the scratch buffer is too small");
   VerifyArgs a{logits, draft, drafts, row_start, temperature, uniform, accepted, tokens, stride, draft_stride, n, rows, vocab,
-               (vocab + CHUNK - 1) / CHUNK, nullptr, nullptr, nullptr, nullptr, nullptr};
+               (vocab + CHUNK - 1) / CHUNK, 1, nullptr, nullptr, nullptr, nullptr, nullptr};
   char* p = (char*)scratch;
   const size_t parts = all * a.chunks;
   a.sum = (double*)p;
@@ -502,7 +509,10 @@ extern "C" int llmlab_verify_drafts(const float* logits, size_t stride, const fl
   a.arrived = a.best + parts;
   hipLaunchKernelGGL(verify_chunks_kernel, dim3(a.chunks, (unsigned)all), dim3(THREADS), 0, stream, a);
   LLMLAB_LAUNCH_CHECK("verify_drafts(chunks)");
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(a.chunks, n), dim3(THREADS), 0, stream, a);
+  // Two chunks a block once there are more blocks than the chip holds at a time, five a unit: the decision is made half as often
+  // (us, one / two, with the draft's logits and without: 32 requests of 152,064 55 / 55 and 38 / 37, 48 77 / 77 and 53 / 48, 64 97 / 93 and 63 / 57).
+  a.each = (long)a.chunks * n > 5 * 256 ? 2 : 1;
+  hipLaunchKernelGGL(verify_draw_kernel, dim3((a.chunks + a.each - 1) / a.each, n), dim3(THREADS), 0, stream, a);
   LLMLAB_LAUNCH_CHECK("verify_drafts(draw)");
   return 0;
 }

@@ -50,6 +50,13 @@ def test_a_vocabulary_of_many_chunks(ops):      # noqa: F811
         assert run(ops, *case) == plain.verify(*case)
 
 
+def test_many_requests_of_many_chunks(ops):      # noqa: F811
+    """More chunks of all requests than the chip holds blocks at a time; the last block of a request has one chunk less."""
+    for with_draft in (False, True):
+        case = inputs([1] * 62 + [0, 2], 23 * 4096 - 5, 3, with_draft, greedy_every=7)
+        assert run(ops, *case) == plain.verify(*case)
+
+
 def test_single_numbers_that_are_none(ops):      # noqa: F811
     """A drafted token's own logit: not a number in the draft's row (its q is zero: it stands), in the target's (its p is: it falls);
     plus infinity, of which no distribution is made."""
