@@ -426,7 +426,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 //
 // What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
 // instructions (512 clocks of a SIMD) and some 170 others (680 and more), 64 of them conversions; three portions of 1,000 tokens behind
-// 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 161 to 172 us (0.75 PFLOP/s), with half of the clocks in vector and a quarter in matrix
+// 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 161 to 172 us (0.70 to 0.75 PFLOP/s), with half of the clocks in vector and a quarter in matrix
 // instructions, and a fifth of the units idle in the last round of blocks.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
 // loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
 // 2^-16 of the sum of sizes), so not used.
