@@ -84,6 +84,22 @@ __device__ __forceinline__ void write_output(const Args& a, int row, int head, i
   for (int j = 0; j < 4; ++j) out[j] = from_float<T>(any ? sum[j] / weight : 0.f);
 }
 
+// The request that is the number-th by the length of its context, the longest first (at most 64 requests; every lane the same)
+struct Request {
+  int b, r0, count, before;
+};
+__device__ __forceinline__ Request longest(const Args& a, int number) {
+  const int lane = threadIdx.x & 63, i = min(lane, a.reqs - 1);
+  const int start = a.q_start[i], rows = a.q_start[i + 1] - start, past = a.start_pos[i], end = past + rows;
+  int ahead = 0;      // requests in front of the lane's
+  for (int j = 0; j < a.reqs; ++j) {
+    const int other = __builtin_amdgcn_readlane(end, j);
+    ahead += other > end || (other == end && j < lane);
+  }
+  const int b = __ffsll(__ballot(lane < a.reqs && ahead == number)) - 1;
+  return Request{b, __builtin_amdgcn_readlane(start, b), __builtin_amdgcn_readlane(rows, b), __builtin_amdgcn_readlane(past, b)};
+}
+
 template <typename T>
 constexpr int parts_of() { return std::is_same<T, float>::value ? 3 : 1; }
 
@@ -292,7 +308,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.z, kvh = blockIdx.y / a.splits, part = blockIdx.y % a.splits, G = a.nq / a.nkv;
   const int r0 = a.q_start[b], count = a.q_start[b + 1] - r0, before = a.start_pos[b];
-  const int total = count * G, row0 = blockIdx.x * TR;
+  const int total = count * G, row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * TR;      // (the longest histories first)
   if (row0 >= total || r0 < 0 || count > a.rows - r0) return;
   const int last = min(row0 + TR, total) - 1;
   const int P = 1 << a.page_shift;
@@ -426,8 +442,8 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 //
 // What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
 // instructions (512 clocks of a SIMD) and some 170 others (680 and more), 64 of them conversions; three portions of 1,000 tokens behind
-// 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 161 to 172 us (0.70 to 0.75 PFLOP/s), with half of the clocks in vector and a quarter in matrix
-// instructions, and a fifth of the units idle in the last round of blocks.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
+// up to 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 149 to 159 us (0.76 to 0.81 PFLOP/s), 62 % of the clocks in vector and 35 % in
+// matrix instructions, a sixth without a block.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
 // loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
 // 2^-16 of the sum of sizes), so not used.
 #define STAGED (HEAD_DIM <= 128)
@@ -466,7 +482,7 @@ struct StagedSizes {
 };
 
 template <int RT, int P>
-__global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles) {
+__global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles, int by_requests) {
   typedef StagedSizes<RT, P> Z;
   constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DJ = (DK + 1) / 2;
   constexpr int PIECES = KT / 16 * PB;                           // loads of 1 KB of a stage's keys, and of its values
@@ -479,15 +495,29 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rt = wave % RT, ph = wave / RT, col = lane & 31, h = lane >> 5, odd = (lane >> 4) & 1, c = lane & 15;
   const int G = a.nq / a.nkv;
-  // the tiles with the longest histories of all kv heads and requests first (or along y and z)
-  int b = blockIdx.z, kvh = blockIdx.y, rank = blockIdx.x;
-  if (gridDim.y == 1 && gridDim.z == 1) {
-    const int per = a.nkv * a.reqs, at = rank % per;
-    rank /= per;
+  // The tiles with the longest histories first, so that the short ones fill what those leave: by tiles, or, where what is before the
+  // portions decides, by requests, those with the longest contexts first (more blocks than x takes: tiles, kv heads, requests)
+  int b = blockIdx.z, kvh = blockIdx.y, rank = blockIdx.x, r0, count, before;
+  if (by_requests) {
+    const int per = tiles * a.nkv, number = rank / per, at = rank - number * per;
+    const Request r = longest(a, number);
+    b = r.b;
+    r0 = r.r0;
+    count = r.count;
+    before = r.before;
     kvh = at % a.nkv;
-    b = at / a.nkv;
+    rank = at / a.nkv;
+  } else {
+    if (gridDim.y == 1 && gridDim.z == 1) {
+      const int per = a.nkv * a.reqs, at = rank % per;
+      rank /= per;
+      kvh = at % a.nkv;
+      b = at / a.nkv;
+    }
+    r0 = a.q_start[b];
+    count = a.q_start[b + 1] - r0;
+    before = a.start_pos[b];
   }
-  const int r0 = a.q_start[b], count = a.q_start[b + 1] - r0, before = a.start_pos[b];
   const int total = count * G, block_row0 = (tiles - 1 - rank) * RT * 32;
   if (block_row0 >= total || r0 < 0 || count > a.rows - r0) return;
   const int row0 = block_row0 + rt * 32, row = row0 + col;
@@ -826,11 +856,12 @@ extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
 extern "C" int llmlab_attention_head_dim() { return D; }
 
 // For measurements and tests: the number of key splits (0: by the rule) and the form of the launch (0: by the rule, else one
-// of those below where it exists)
-static int g_force_splits = 0, g_force_form = 0;
+// of those below where it exists; + 10: its blocks by tiles, + 20: by requests)
+static int g_force_splits = 0, g_force_form = 0, g_force_order = -1;
 extern "C" void llmlab_debug_attention_e4m3(int splits, int form) {
   g_force_splits = splits;
-  g_force_form = form;
+  g_force_form = form % 10;
+  g_force_order = form / 10 - 1;
 }
 
 constexpr int SPLIT_WAVES = 4;
@@ -903,11 +934,16 @@ static int launch_split(Args a, long most_rows, int visible, float* workspace, s
 }
 
 #if STAGED
+// The blocks' order where what is before the portions is half of them or more: by requests, the longest contexts first (us, by tiles / by
+// requests, 28 heads of 128 over 4, contexts from 4 / 9 of the longest on: 3 x 1,000 up to 4,096 160 / 149, 5 x 700 up to 8,192 368 / 320, 2 x 2,000 up to
+// 4,000 195 / 165, 3 x 1,200 up to 1,800 73.7 / 70.7; prompts from their start, 5 x 1,600 87 / 98).
 template <int RT, int P>
-static int launch_staged(const Args& a, long most_rows, hipStream_t stream) {
+static int launch_staged(const Args& a, long most_rows, bool history, hipStream_t stream) {
   const long tiles = (most_rows + 32 * RT - 1) / (32 * RT), blocks = tiles * a.nkv * a.reqs;
-  const dim3 grid = blocks * 64 * RT * P <= 0xffffffffL ? dim3((unsigned)blocks) : dim3((unsigned)tiles, a.nkv, a.reqs);
-  hipLaunchKernelGGL((attention_e4m3_staged_kernel<RT, P>), grid, dim3(64 * RT * P), 0, stream, a, (int)tiles);
+  const bool along_x = blocks * 64 * RT * P <= 0xffffffffL;
+  const dim3 grid = along_x ? dim3((unsigned)blocks) : dim3((unsigned)tiles, a.nkv, a.reqs);
+  const int by_requests = g_force_order >= 0 && a.reqs <= 64 ? g_force_order : along_x && history && a.reqs > 1 && a.reqs <= 64;
+  hipLaunchKernelGGL((attention_e4m3_staged_kernel<RT, P>), grid, dim3(64 * RT * P), 0, stream, a, (int)tiles, by_requests);
   LLMLAB_LAUNCH_CHECK("attention(e4m3, staged)");
   return 0;
 }
@@ -940,10 +976,11 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
     return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 #if STAGED
   const int middle = max_ctx_len - max_q_len / 2, walk = window > 0 ? std::min(window, middle) : middle;
+  const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len;
   const int form = g_force_form > 0 ? g_force_form : launch_form(most_rows, (long)nkv * reqs, walk, visible, num_cus);
-  if (form == FORM_2x4) return launch_staged<2, 4>(a, most_rows, stream);
-  if (form == FORM_2x2) return launch_staged<2, 2>(a, most_rows, stream);
-  if (form == FORM_4x1) return launch_staged<4, 1>(a, most_rows, stream);
+  if (form == FORM_2x4) return launch_staged<2, 4>(a, most_rows, history, stream);
+  if (form == FORM_2x2) return launch_staged<2, 2>(a, most_rows, history, stream);
+  if (form == FORM_4x1) return launch_staged<4, 1>(a, most_rows, history, stream);
 #endif
   return most_rows > 16 && D <= 128 ? launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream)
                                     : launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);

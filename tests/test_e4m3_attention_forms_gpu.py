@@ -99,6 +99,19 @@ def test_one_number_that_is_none(ops, form, d):      # noqa: F811
         assert torch.equal(torch.isnan(got), expect)
 
 
+@pytest.mark.parametrize("form", [12, 22, 23, 24, 20])
+@pytest.mark.parametrize("lengths,counts,window", [
+    ([700, 90, 701, 300], [90, 90, 41, 90], None),
+    ([200] * 64, [21, 1, 0, 33] * 16, None),                        # as many requests as are put in order; equal ones
+    ([65] + [130] * 64, [33] * 65, 90),                             # one more
+    ([40, 900, 33], [40, 0, 33], None),                             # the longest has no tokens
+])
+def test_orders_of_blocks(ops, form, lengths, counts, window):      # noqa: F811
+    """By tiles, and by requests with the longest contexts first: every row once, whatever the order."""
+    with ops.debug.force(e4m3_attention=(64, 0, form)):
+        check(ops, 6, 2, 64, 16, lengths, counts, "bf16", window, seed=form)
+
+
 @pytest.mark.parametrize("splits", [1, 2, 7, 64])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_key_splits(ops, splits, dtype):      # noqa: F811
