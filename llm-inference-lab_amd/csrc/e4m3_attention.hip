@@ -78,10 +78,13 @@ struct Args {
 // Four numbers of a row's output: its sums over the sum of its probabilities, zero where it saw no key.
 template <typename T>
 __device__ __forceinline__ void write_output(const Args& a, int row, int head, int i, floatx4 sum, float weight) {
-  T* out = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + i;
+  typedef T vec __attribute__((ext_vector_type(4)));      // (outputs begin at 16 bytes, and their rows)
   const bool any = weight > 0.f || weight != weight;
+  const float inv = 1.f / weight;
+  vec v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] = from_float<T>(any ? sum[j] / weight : 0.f);
+  for (int j = 0; j < 4; ++j) v[j] = from_float<T>(!any ? 0.f : sizeof(T) == 4 ? sum[j] / weight : sum[j] * inv);
+  *(vec*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + i) = v;
 }
 
 // The request that is the number-th by the length of its context, the longest first (at most 64 requests; every lane the same)
@@ -961,6 +964,8 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   LLMLAB_REQUIRE(reqs >= 0 && reqs <= 65535, "attention(e4m3): %d requests, at most 65535 are taken", reqs);
   LLMLAB_REQUIRE(window >= 0, "attention(e4m3): negative window");
   LLMLAB_REQUIRE(scale > 0.f, "attention(e4m3): the score scale must be positive, got %g", (double)scale);
+  LLMLAB_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)out % 16) == 0 && q_stride % (dtype == DT_F32 ? 4 : 8) == 0 && out_stride % 8 == 0,
+                 "attention(e4m3): queries and outputs are not aligned for vector loads");
   LLMLAB_REQUIRE(((uintptr_t)k % 16) == 0 && ((uintptr_t)v % 16) == 0 && ((uintptr_t)kv_scale % 4) == 0,
                  "attention(e4m3): the pages are not aligned for vector loads");
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;

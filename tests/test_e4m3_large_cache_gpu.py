@@ -79,3 +79,20 @@ def test_key_splits_in_a_graph(ops, dtype):      # noqa: F811
         ops.workspace.fill_(float("nan"))
         torch.cuda.synchronize()
         assert torch.equal(out, again)
+
+
+def test_queries_at_the_least_stride_and_place(ops):      # noqa: F811
+    """float32 queries whose rows are 4 numbers apart from a multiple of 8, bfloat16 ones 8: what 16-byte loads can take."""
+    nq, nkv, d, page = 4, 2, 64, 64
+    lengths, counts = [90, 300], [1, 40]
+    cache = Cache(lengths, nkv, d, page).fill()
+    q_start, start_pos, _, _ = ragged(lengths, counts)
+    for dtype, more in (("f32", 4), ("bf16", 8)):
+        q = queries(41, nq, d, dtype, 1)
+        wide = torch.zeros((41, nq * d + more), dtype=DTYPES[dtype])
+        wide[:, more:] = q
+        dev = cache.on(DEVICE)
+        out = torch.zeros((41, nq * d), dtype=DTYPES[dtype], device=DEVICE)
+        ops.paged_attention_e4m3(wide.to(DEVICE)[:, more:], nq, nkv, d, dev.k, dev.v, dev.scale, dev.table, page, q_start.to(DEVICE),
+                                 start_pos.to(DEVICE), 2, 40, 300, None, 0.002, out)
+        assert torch.equal(out.cpu(), run(ops, cache, q, nq, q_start, start_pos, lengths, counts, None, 0.002))
