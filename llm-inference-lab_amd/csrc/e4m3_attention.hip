@@ -429,7 +429,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 }
 
 // ------------------------------------------------------------- many rows, codes staged in LDS
-// bfloat16 rows at heads up to 128.  A block has RT tiles of 32 rows side by side, and P groups of waves that
+// Heads up to 128.  A block has RT tiles of 32 rows side by side, and P groups of waves that
 // take the staged keys in turn, 32 of every 32 P; the groups' sums meet in LDS at the end.  The codes come by direct loads
 // into LDS, in the cache's order, in two stages, one being multiplied while the other is on its way, one barrier a
 // stage, and become bfloat16 numbers behind the read from LDS: half the bytes there and on the way.  Products by
@@ -448,7 +448,8 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 // up to 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 149 to 159 us (0.76 to 0.81 PFLOP/s), 62 % of the clocks in vector and 35 % in
 // matrix instructions, a sixth without a block.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
 // loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
-// 2^-16 of the sum of sizes), so not used.
+// 2^-16 of the sum of sizes), so not used.  float32 rows take three products a part of what they read, and as many conversions of codes as one:
+// 7 requests of 700 tokens, 56 heads of 128 over 8, up to 1,400 keys 273 us (split over waves 439).
 #define STAGED (HEAD_DIM <= 128)
 #if STAGED
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
@@ -484,9 +485,17 @@ struct StagedSizes {
   static constexpr int LDS = (STAGES > SUMS ? STAGES : SUMS) + NW * 32 * 4 * 3;
 };
 
-template <int RT, int P>
-__global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 : 2) void attention_e4m3_staged_kernel(Args a, int tiles, int by_requests) {
+// The waves that a SIMD is to hold, as many as fit without a spilled register
+constexpr int staged_waves(int parts, int groups) {
+  if (parts > 1) return D <= 64 ? 3 : 2;
+  return D <= 64 ? 4 : groups < 4 && REST != 3 ? 3 : 2;
+}
+
+template <typename T, int RT, int P>
+__global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void attention_e4m3_staged_kernel(Args a, int tiles,
+                                                                                                           int by_requests) {
   typedef StagedSizes<RT, P> Z;
+  constexpr int PARTS = parts_of<T>();
   constexpr int NW = Z::NW, KT = Z::KT, DK = D / 16, DJ = (DK + 1) / 2;
   constexpr int PIECES = KT / 16 * PB;                           // loads of 1 KB of a stage's keys, and of its values
   constexpr int EACH = PIECES * 2 / NW;                          // ... of a wave
@@ -595,20 +604,38 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
     return there;
   };
 
-  bf16x8 q[2 * DJ];
-  {
-    const bf16_t* qp = (const bf16_t*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
+  // (a sixteen past the last: its keys' last one, times zero)
+  bf16x8 q[PARTS][2 * DJ];
+  const T* qp = (const T*)a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * D;
+  auto in = [&](int k) { return valid && (DK % 2 == 0 || (k >> 1) * 2 + h < DK); };
+  auto at = [&](int k) { return qp + min((k >> 1) * 2 + h, DK - 1) * 16 + (k & 1) * 8; };
+  if constexpr (PARTS == 1) {
 #pragma unroll
-    for (int k = 0; k < 2 * DJ; ++k) q[k] = *(const bf16x8*)(qp + min((k >> 1) * 2 + h, DK - 1) * 16 + (k & 1) * 8);
+    for (int k = 0; k < 2 * DJ; ++k) q[0][k] = *(const bf16x8*)at(k);
+    locate(tile_lo);
+  } else {
+    locate(tile_lo);
+#pragma unroll
+    for (int k = 0; k < 2 * DJ; ++k) {
+      const floatx4 x = *(const floatx4*)at(k), y = *(const floatx4*)(at(k) + 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bf16_t part[PARTS];
+        split<PARTS>(i < 4 ? x[i & 3] : y[i & 3], part);
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) q[n][k][i] = part[n];
+      }
+    }
   }
-  locate(tile_lo);
   // (waited for here, with the table: in the loop it would be waited for, with all that is on its way, in every step)
 #pragma unroll
-  for (int k = 0; k < 2 * DJ; ++k) {
-    const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-    q[k] = valid && (DK % 2 == 0 || (k >> 1) * 2 + h < DK) ? q[k] : zero;      // (a sixteen past the last: its keys' last one, times zero)
-    asm volatile("" : "+v"(q[k]));
-  }
+  for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+    for (int k = 0; k < 2 * DJ; ++k) {
+      const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+      q[n][k] = in(k) ? q[n][k] : zero;
+      asm volatile("" : "+v"(q[n][k]));
+    }
   floatx16 o[DV];
 #pragma unroll
   for (int i = 0; i < DV; ++i)
@@ -644,8 +671,12 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
     for (int x = 0; x < 16; ++x) s[x] = 0.f;
 #pragma unroll
     for (int j = 0; j < DJ; ++j) {
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][0], kc[j][1], ks), q[2 * j], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(kc[j][2], kc[j][3], ks), q[2 * j + 1], s, 0, 0, 0);
+      const bf16x8 k0 = eight_numbers(kc[j][0], kc[j][1], ks), k1 = eight_numbers(kc[j][2], kc[j][3], ks);
+#pragma unroll
+      for (int n = PARTS - 1; n >= 0; --n) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, q[n][2 * j], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, q[n][2 * j + 1], s, 0, 0, 0);
+      }
     }
     // the values' codes travel while the maximum is found: [block of 16][group of 64][quad h or 2 + h], two blocks of 16 of d each
     typedef unsigned uint2v __attribute__((ext_vector_type(2)));
@@ -731,15 +762,23 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
       for (int i = 0; i < 8; ++i) p[i] = fast_exp2(fmaf(s[block * 8 + i], a.scale2, neg_m));
       l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       const floatx4 w0 = *(const floatx4*)(own_scales + block * 16 + 4 * h), w1 = *(const floatx4*)(own_scales + block * 16 + 8 + 4 * h);
-      bf16x8 pf;
+      bf16x8 pf[PARTS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pf[i] = (bf16_t)(p[i] * (i < 4 ? w0[i & 3] : w1[i & 3]));
+      for (int i = 0; i < 8; ++i) {
+        bf16_t part[PARTS];
+        split<PARTS>(p[i] * (i < 4 ? w0[i & 3] : w1[i & 3]), part);
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) pf[n][i] = part[n];
+      }
 #pragma unroll
       for (int group = 0; group < GROUPS; ++group)
 #pragma unroll
-        for (int i = 0; i < (group < FULL ? 2 : REST_DV); ++i)
-          o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_numbers(vc[block][group][0][i], vc[block][group][1][i], 1.f), pf,
-                                                                     o[group * 2 + i], 0, 0, 0);
+        for (int i = 0; i < (group < FULL ? 2 : REST_DV); ++i) {
+          const bf16x8 vf = eight_numbers(vc[block][group][0][i], vc[block][group][1][i], 1.f);
+#pragma unroll
+          for (int n = PARTS - 1; n >= 0; --n)
+            o[group * 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[n], o[group * 2 + i], 0, 0, 0);
+        }
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);      // the last loads (of a tile past the end) are in, and the stages read
@@ -762,7 +801,7 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
     if (has_row)
 #pragma unroll
       for (int n = 0; n < DV * 4; ++n)
-        if (place(n) >= 0) write_output<bf16_t>(a, r0 + out_tok, out_head, place(n), piece(n), l);
+        if (place(n) >= 0) write_output<T>(a, r0 + out_tok, out_head, place(n), piece(n), l);
   } else {
     // group ph puts the pieces ph, ph + P, .. of its rows together; the others' it finds in LDS
     constexpr int SHARES = DV * 4 / P;
@@ -802,7 +841,7 @@ __global__ __launch_bounds__(64 * RT * P, D <= 64 ? 4 : P < 4 && REST != 3 ? 3 :
       for (int p = 0; p < P; ++p)
         v += w[p] * (p == ph ? mine[n] : left[(((p * RT + rt) * SHARES + n) * (P - 1) + (ph > p ? ph - 1 : ph)) * 64 + lane]);
       const int to = place(n * P + ph);
-      if (has_row && to >= 0) write_output<bf16_t>(a, r0 + out_tok, out_head, to, v, weight);
+      if (has_row && to >= 0) write_output<T>(a, r0 + out_tok, out_head, to, v, weight);
     }
   }
 }
@@ -877,7 +916,7 @@ static int key_splits(long blocks, int visible, int num_cus) {
   return (int)std::max(1L, std::min(std::min(2L * num_cus / blocks, most), 128L));
 }
 
-// The form of a bfloat16 launch at heads up to 128: the one whose time is the least by an estimate, rounds of blocks (`more`
+// The form of a launch at heads up to 128, of bfloat16 rows: the one whose time is the least by an estimate, rounds of blocks (`more`
 // for the last one's part and for what uneven tiles leave, `least` where units have few blocks) x (a block's start and end +
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
@@ -887,28 +926,43 @@ static int key_splits(long blocks, int visible, int num_cus) {
 // us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
 // of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
 // 1,304 of 40 behind 63 32 / 38 / 26 / 21.5; 6,624 of 48 behind 232 241 / 269 / 161 / 148.
+//
+// float32 rows likewise, without 2x4 (which no launch of 80 drawn was fastest in): fitted to 700 launches, over 600 others the
+// picks lose 0.7 % to the best (39 % at worst), and gain 11 % (heads of 64) and 14 % (128) on the split form, up to 2.6 times.  us, split / 2x2 / 4x1: 1,500 tokens of 32
+// heads of 128 over 8 behind 3,000 keys 315 / 239 / 276; 7 requests of 700 tokens, 56 over 8, behind 700 439 / 290 / 273; 16 of 128, 32 over 8,
+// behind 100 58 / 39 / 31; 61 tokens of 16 heads over 2 through a window of 1,000 24 / 36 / 56.
 enum { FORM_SPLIT = 1, FORM_2x4, FORM_2x2, FORM_4x1 };
 #if STAGED
+struct Form {
+  int form, rows, groups;
+  float blocks_a_unit, start, step, more, least;
+};
+template <typename T>
 static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
   if (most_rows <= 16) return FORM_SPLIT;
-  struct Form { int rows, groups; float blocks_a_unit, start, step, more, least; };
-  constexpr Form forms[] = {{32, SPLIT_WAVES, D <= 64 ? 3.f : 2.f, D <= 64 ? 5.5f : 6.4f, D <= 64 ? 1.14f : 1.18f, D <= 64 ? .54f : .58f, D <= 64 ? .79f : .92f},
-                            {64, 4, D <= 64 ? 2.f : 1.f, D <= 64 ? 6.f : 8.2f, D <= 64 ? .85f : 1.18f, D <= 64 ? .9f : .34f, D <= 64 ? .83f : 1.f},
-                            {64, 2, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.2f : 10.5f, D <= 64 ? .75f : 1.06f, D <= 64 ? .82f : .51f, .71f},
-                            {128, 1, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.7f : 10.4f, D <= 64 ? .63f : .97f, D <= 64 ? .95f : .72f, D <= 64 ? .71f : .8f}};
-  constexpr float MERGE = D <= 64 ? 2.2f : 1.3f;
+  constexpr bool F32 = parts_of<T>() > 1;
+  constexpr Form bf16_forms[] = {
+      {FORM_SPLIT, 32, SPLIT_WAVES, D <= 64 ? 3.f : 2.f, D <= 64 ? 5.5f : 6.4f, D <= 64 ? 1.14f : 1.18f, D <= 64 ? .54f : .58f, D <= 64 ? .79f : .92f},
+      {FORM_2x4, 64, 4, D <= 64 ? 2.f : 1.f, D <= 64 ? 6.f : 8.2f, D <= 64 ? .85f : 1.18f, D <= 64 ? .9f : .34f, D <= 64 ? .83f : 1.f},
+      {FORM_2x2, 64, 2, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.2f : 10.5f, D <= 64 ? .75f : 1.06f, D <= 64 ? .82f : .51f, .71f},
+      {FORM_4x1, 128, 1, D <= 64 ? 4.f : 3.f, D <= 64 ? 6.7f : 10.4f, D <= 64 ? .63f : .97f, D <= 64 ? .95f : .72f, D <= 64 ? .71f : .8f}};
+  constexpr Form f32_forms[] = {
+      {FORM_SPLIT, 16, SPLIT_WAVES, D <= 64 ? 3.f : 2.f, D <= 64 ? 4.2f : 4.9f, D <= 64 ? 1.28f : 1.35f, D <= 64 ? .61f : .52f, D <= 64 ? .83f : .91f},
+      {FORM_2x2, 64, 2, D <= 64 ? 3.f : 2.f, D <= 64 ? 8.4f : 10.7f, D <= 64 ? 1.27f : 1.62f, D <= 64 ? .71f : .57f, D <= 64 ? .34f : .82f},
+      {FORM_4x1, 128, 1, D <= 64 ? 3.f : 2.f, D <= 64 ? 8.1f : 9.8f, D <= 64 ? 1.23f : 1.62f, D <= 64 ? .8f : .77f, D <= 64 ? .78f : .74f}};
+  constexpr float MERGE = F32 ? (D <= 64 ? 2.6f : .6f) : D <= 64 ? 2.2f : 1.3f;
   int best = 0;
   float least = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    const Form& f = forms[i];
+  for (int i = 0; i < (F32 ? 3 : 4); ++i) {
+    const Form& f = F32 ? f32_forms[i < 3 ? i : 0] : bf16_forms[i];
     const long tiles = (most_rows + f.rows - 1) / f.rows * pairs;
-    const int splits = i == 0 ? key_splits(tiles, visible, num_cus) : 1;
+    const int splits = f.form == FORM_SPLIT ? key_splits(tiles, visible, num_cus) : 1;
     const float steps = splits > 1 ? (float)visible / (32 * f.groups * splits) : (float)walk / (32 * f.groups);
     const float rounds = (float)tiles * splits / (f.blocks_a_unit * num_cus) + f.more;
     const float time = std::max(rounds, f.least) * (f.start + std::max(steps, 1.f) * f.step) + (splits > 1 ? MERGE : 0.f);
     if (i == 0 || time < least) {
       least = time;
-      best = i + 1;
+      best = f.form;
     }
   }
   return best;
@@ -940,13 +994,13 @@ static int launch_split(Args a, long most_rows, int visible, float* workspace, s
 // The blocks' order where what is before the portions is half of them or more: by requests, the longest contexts first (us, by tiles / by
 // requests, 28 heads of 128 over 4, contexts from 4 / 9 of the longest on: 3 x 1,000 up to 4,096 160 / 149, 5 x 700 up to 8,192 368 / 320, 2 x 2,000 up to
 // 4,000 195 / 165, 3 x 1,200 up to 1,800 73.7 / 70.7; prompts from their start, 5 x 1,600 87 / 98).
-template <int RT, int P>
+template <typename T, int RT, int P>
 static int launch_staged(const Args& a, long most_rows, bool history, hipStream_t stream) {
   const long tiles = (most_rows + 32 * RT - 1) / (32 * RT), blocks = tiles * a.nkv * a.reqs;
   const bool along_x = blocks * 64 * RT * P <= 0xffffffffL;
   const dim3 grid = along_x ? dim3((unsigned)blocks) : dim3((unsigned)tiles, a.nkv, a.reqs);
   const int by_requests = g_force_order >= 0 && a.reqs <= 64 ? g_force_order : along_x && history && a.reqs > 1 && a.reqs <= 64;
-  hipLaunchKernelGGL((attention_e4m3_staged_kernel<RT, P>), grid, dim3(64 * RT * P), 0, stream, a, (int)tiles, by_requests);
+  hipLaunchKernelGGL((attention_e4m3_staged_kernel<T, RT, P>), grid, dim3(64 * RT * P), 0, stream, a, (int)tiles, by_requests);
   LLMLAB_LAUNCH_CHECK("attention(e4m3, staged)");
   return 0;
 }
@@ -977,16 +1031,20 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
   const int visible = window > 0 ? (int)std::min((long)max_ctx_len, (long)window + max_q_len) : max_ctx_len;
   if (num_cus <= 0) num_cus = 256;
-  if (dtype == DT_F32)
-    return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 #if STAGED
   const int middle = max_ctx_len - max_q_len / 2, walk = window > 0 ? std::min(window, middle) : middle;
-  const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len;
-  const int form = g_force_form > 0 ? g_force_form : launch_form(most_rows, (long)nkv * reqs, walk, visible, num_cus);
-  if (form == FORM_2x4) return launch_staged<2, 4>(a, most_rows, history, stream);
-  if (form == FORM_2x2) return launch_staged<2, 2>(a, most_rows, history, stream);
-  if (form == FORM_4x1) return launch_staged<4, 1>(a, most_rows, history, stream);
+  const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len, f32 = dtype == DT_F32;
+  const int form = g_force_form > 0 ? g_force_form
+                   : f32            ? launch_form<float>(most_rows, (long)nkv * reqs, walk, visible, num_cus)
+                                    : launch_form<bf16_t>(most_rows, (long)nkv * reqs, walk, visible, num_cus);
+  if (form == FORM_2x4 && !f32) return launch_staged<bf16_t, 2, 4>(a, most_rows, history, stream);
+  if (form == FORM_2x2)
+    return f32 ? launch_staged<float, 2, 2>(a, most_rows, history, stream) : launch_staged<bf16_t, 2, 2>(a, most_rows, history, stream);
+  if (form == FORM_4x1)
+    return f32 ? launch_staged<float, 4, 1>(a, most_rows, history, stream) : launch_staged<bf16_t, 4, 1>(a, most_rows, history, stream);
 #endif
+  if (dtype == DT_F32)
+    return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
   return most_rows > 16 && D <= 128 ? launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream)
                                     : launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 }

@@ -148,9 +148,9 @@ class KernelDebug:
         where one launch would serve both, or one launch wherever there is a kernel for both; ``attention_small_tiles``:
         a head size (up to 128); one launch with the portions by tiles of 16 rows.
         ``e4m3_attention``: (head size, key splits, form) of attention over 8-bit keys and values: 0 splits as the kernel
-        chooses; form 0 as it chooses, 1 = the waves of a block split the keys of a tile, and at heads up to 128 in bfloat16
-        2 to 4 = keys staged in LDS, blocks of 2 tiles of 32 rows by 4 groups of waves, 2 by 2, 4 by 1 (+ 10: their blocks by
-        tiles, + 20: by requests).
+        chooses; form 0 as it chooses, 1 = the waves of a block split the keys of a tile, and at heads up to 128
+        2 to 4 = keys staged in LDS, blocks of 2 tiles of 32 rows by 4 groups of waves (not in float32), 2 by 2, 4 by 1 (+ 10:
+        their blocks by tiles, + 20: by requests).
         ``f32_fma``: float32 products of many rows by the plain FMA kernel instead of the
         matrix cores.  Other keywords: fields of ``DispatchRules`` for the time of the block."""
         ops = self._ops

@@ -112,6 +112,47 @@ def test_orders_of_blocks(ops, form, lengths, counts, window):      # noqa: F811
         check(ops, 6, 2, 64, 16, lengths, counts, "bf16", window, seed=form)
 
 
+@pytest.mark.parametrize("form", [0, 3, 4])
+@pytest.mark.parametrize("d", [16, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("nq,nkv,page,lengths,counts,window", [
+    (1, 1, 16, [1], [1], None),
+    (4, 2, 64, [1, 64, 65, 127, 300], [1, 1, 1, 65, 1], None),
+    (12, 2, 64, [300, 300], [1, 50], 64),
+    (4, 4, 64, [400], [3], 1),
+    (2, 1, 16, [16 * 300 + 5], [37], None),                         # more tiles than a wave looks up pages for at a time
+    (16, 2, 16, [700, 300], [129, 50], 200),
+])
+def test_forms_in_float32(ops, form, d, nq, nkv, page, lengths, counts, window):      # noqa: F811
+    with ops.debug.force(e4m3_attention=(d, 0, form)):
+        check(ops, nq, nkv, d, page, lengths, counts, "f32", window, seed=form)
+
+
+@pytest.mark.parametrize("form", [3, 4])
+def test_what_stays_with_its_rows_in_float32(ops, form):      # noqa: F811
+    with ops.debug.force(e4m3_attention=(64, 0, form)):
+        for counts in ([4], [70]):
+            whole.test_what_is_not_a_number_stays_with_the_rows_that_see_it(ops, "f32", counts)
+
+
+@pytest.mark.parametrize("form", [13, 14, 23, 24])
+def test_orders_of_blocks_in_float32(ops, form):      # noqa: F811
+    with ops.debug.force(e4m3_attention=(128, 0, form)):
+        check(ops, 6, 2, 128, 16, [700, 90, 701, 300], [90, 90, 41, 90], "f32", None, seed=form)
+
+
+def test_many_float32_rows(ops):      # noqa: F811
+    """As many as take the codes staged in LDS without a form forced; the same bits every time."""
+    nq, nkv, d, page = 32, 4, 128, 64
+    lengths, counts = [260, 400, 300, 260], [256, 200, 256, 33]
+    check(ops, nq, nkv, d, page, lengths, counts, "f32", None, seed=3)
+    cache = Cache(lengths, nkv, d, page).fill()
+    q_start, start_pos, positions, _ = ragged(lengths, counts)
+    q = queries(len(positions), nq, d, "f32", 1)
+    dev = cache.on(whole.DEVICE)
+    outs = [run(ops, cache, q, nq, q_start, start_pos, lengths, counts, None, 0.002, dev=dev) for _ in range(3)]
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
 @pytest.mark.parametrize("splits", [1, 2, 7, 64])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_key_splits(ops, splits, dtype):      # noqa: F811

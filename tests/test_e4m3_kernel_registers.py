@@ -5,7 +5,8 @@ from llm_inference_lab_amd.kernels import build
 from test_kernel_registers import SIMD_REGISTERS, kernels, library
 
 
-@pytest.mark.parametrize("d,kernel,waves,least", [(64, "e4m3_staged", 4, 3), (128, "e4m3_staged", 2, 3), (64, "e4m3_split", 2, 3),
+@pytest.mark.parametrize("d,kernel,waves,least", [(64, "e4m3_staged_kernelIDF16b", 4, 3), (128, "e4m3_staged_kernelIDF16b", 2, 3),
+                                                  (64, "e4m3_staged_kernelIf", 3, 2), (128, "e4m3_staged_kernelIf", 2, 2), (64, "e4m3_split", 2, 3),
                                                   (128, "e4m3_split", 2, 3)])
 def test_waves_a_simd_holds(d, kernel, waves, least):
     taken = {name: v for name, v in kernels(library(lambda: build.e4m3_attention_library(d))).items() if kernel in name}
