@@ -68,7 +68,7 @@ struct Args {
   void* out;                   // [rows, out_stride]
   long q_stride, out_stride;
   int table_stride, table_width, page_shift, pages;
-  int last_key;                // the last that the table has room for
+  int last_key;                // the last that the table has room for (-1: no walk, nothing of the cache is read)
   int nq, nkv, window, rows, reqs, splits;
   float scale2;                // the scores' factor times log2 e
   float* o_part;               // [rows * nq, splits, D]    (splits > 1)
@@ -1017,6 +1017,7 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   LLMLAB_REQUIRE(q_stride >= (long)nq * D && out_stride >= (long)nq * D, "attention(e4m3): row strides too small");
   LLMLAB_REQUIRE(reqs >= 0 && reqs <= 65535, "attention(e4m3): %d requests, at most 65535 are taken", reqs);
   LLMLAB_REQUIRE(window >= 0, "attention(e4m3): negative window");
+  LLMLAB_REQUIRE(pages >= 0 && table_width >= 0, "attention(e4m3): %d pages, a block table of %d", pages, table_width);
   LLMLAB_REQUIRE(scale > 0.f, "attention(e4m3): the score scale must be positive, got %g", (double)scale);
   LLMLAB_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)out % 16) == 0 && q_stride % (dtype == DT_F32 ? 4 : 8) == 0 && out_stride % 8 == 0,
                  "attention(e4m3): queries and outputs are not aligned for vector loads");
@@ -1025,7 +1026,7 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;
   Args a{q, (const unsigned char*)k, (const unsigned char*)v, (const unsigned char*)kv_scale, table, q_start, start_pos, out,
          q_stride, out_stride, table_stride, table_width, 0, pages,
-         (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
+         pages == 0 ? -1 : (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
          nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
@@ -1034,9 +1035,12 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
 #if STAGED
   const int middle = max_ctx_len - max_q_len / 2, walk = window > 0 ? std::min(window, middle) : middle;
   const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len, f32 = dtype == DT_F32;
-  const int form = g_force_form > 0 ? g_force_form
-                   : f32            ? launch_form<float>(most_rows, (long)nkv * reqs, walk, visible, num_cus)
-                                    : launch_form<bf16_t>(most_rows, (long)nkv * reqs, walk, visible, num_cus);
+  // (a cache without pages: nothing there to be read in the place of a missing page.  With no last key the split form walks no step and
+  // the rows are zeros; the staged forms read a stage in any case.)
+  const int form = pages == 0         ? (int)FORM_SPLIT
+                   : g_force_form > 0 ? g_force_form
+                   : f32              ? launch_form<float>(most_rows, (long)nkv * reqs, walk, visible, num_cus)
+                                      : launch_form<bf16_t>(most_rows, (long)nkv * reqs, walk, visible, num_cus);
   if (form == FORM_2x4 && !f32) return launch_staged<bf16_t, 2, 4>(a, most_rows, history, stream);
   if (form == FORM_2x2)
     return f32 ? launch_staged<float, 2, 2>(a, most_rows, history, stream) : launch_staged<bf16_t, 2, 2>(a, most_rows, history, stream);
