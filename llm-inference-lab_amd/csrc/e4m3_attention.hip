@@ -70,6 +70,7 @@ struct Args {
   int table_stride, table_width, page_shift, pages;
   int last_key;                // the last that the table has room for (-1: no walk, nothing of the cache is read)
   int nq, nkv, window, rows, reqs, splits;
+  int covered;                 // rows (token, head of a group) of a request that the launch has tiles for
   float scale2;                // the scores' factor times log2 e
   float* o_part;               // [rows * nq, splits, D]    (splits > 1)
   float* ml_part;              // [rows * nq, splits, 2]
@@ -848,13 +849,14 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
 #endif  // STAGED
 
 // The splits of a row put together: a wave a (row, head), four numbers a lane and, where a head leaves lanes over, several splits at a
-// time.  All of up to 8 splits a group of lanes are on their way while the factors are worked out (a lane a split).
+// time.  All of up to 8 splits a group of lanes are on their way while the factors are worked out (a lane a split) and the row's request is
+// found: a row that the first launch left alone (of no request, of one whose starts do not fit the rows, or behind its tiles) stays as it is.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
   constexpr int LANES = D / 4, GROUPS = 64 % LANES == 0 ? 64 / LANES : 1, AT_ONCE = 8;
-  const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int row = at / a.nq;
-  if (row < a.q_start[0] || row >= a.q_start[a.reqs] || row >= a.rows) return;
+  const int at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = at / a.nq, head = at - row * a.nq;
+  if (row >= a.rows) return;
   const int group = lane / LANES < GROUPS ? lane / LANES : 0, i = GROUPS > 1 ? lane % LANES * 4 : lane * 4;
   const float* ml = a.ml_part + (size_t)at * a.splits * 2;
   const float* o = a.o_part + (size_t)at * a.splits * D + (i < D ? i : 0);
@@ -871,6 +873,18 @@ __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
     m[n] = s < a.splits ? ml[2 * s] : NEG_INF;
     w[n] = s < a.splits ? ml[2 * s + 1] : 0.f;
   }
+  int r0 = -1, end = 0;      // of the last request that begins at or before the row
+  for (int base = 0; base < a.reqs; base += 64) {
+    const int i = min(base + lane, a.reqs - 1), start = a.q_start[i], next = a.q_start[i + 1];
+    const unsigned long long begun = __ballot(base + lane < a.reqs && start <= row);
+    if (begun) {
+      const int last = 63 - __clzll(begun);
+      r0 = __builtin_amdgcn_readlane(start, last);
+      end = __builtin_amdgcn_readlane(next, last);
+    }
+  }
+  const int G = a.nq / a.nkv;
+  if (r0 < 0 || row >= end || end > a.rows || (long)(row - r0) * G + head % G >= a.covered) return;
   const float top = full_wave_max(fmaxf(m[0], m[1]));
 #pragma unroll
   for (int n = 0; n < 2; ++n) f[n] = m[n] == NEG_INF ? 1.f : fast_exp2(m[n] - top);
@@ -891,7 +905,7 @@ __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor(sum[j], off, WAVE);
   }
-  if (GROUPS > 1 ? lane < LANES : i < D) write_output<T>(a, row, at - row * a.nq, i, sum, l);
+  if (GROUPS > 1 ? lane < LANES : i < D) write_output<T>(a, row, head, i, sum, l);
 }
 
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }
@@ -973,6 +987,7 @@ template <typename T, int QB>
 static int launch_split(Args a, long most_rows, int visible, float* workspace, size_t workspace_floats, int num_cus,
                         hipStream_t stream) {
   const long tiles = (most_rows + 16 * QB - 1) / (16 * QB);
+  a.covered = (int)std::min(tiles * 16 * QB, 0x7fffffffL);
   a.splits = g_force_splits > 0 ? g_force_splits : key_splits(tiles * a.nkv * a.reqs, visible, num_cus);
   const size_t each = (size_t)a.rows * a.nq * (D + 2);
   a.splits = (int)std::max((size_t)1, std::min((size_t)std::min(a.splits, 65535 / a.nkv), workspace_floats / std::max(each, (size_t)1)));
@@ -1026,7 +1041,7 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;
   Args a{q, (const unsigned char*)k, (const unsigned char*)v, (const unsigned char*)kv_scale, table, q_start, start_pos, out,
          q_stride, out_stride, table_stride, table_width, 0, pages,
-         pages == 0 ? -1 : (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, scale * 1.4426950408889634f,
+         pages == 0 ? -1 : (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, 0, scale * 1.4426950408889634f,
          nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
