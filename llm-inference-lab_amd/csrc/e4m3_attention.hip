@@ -33,6 +33,7 @@ constexpr int DB = D / 16;               // 16-wide blocks of a value
 constexpr int VG = (DB + 3) / 4;         // groups of four of them
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float LARGE = 1.7014118346046923e38f;      // 2^127
+constexpr float LOWEST = -3.40282347e38f;            // a row's maximum once it saw a key (minus infinity: it saw none)
 constexpr float LAZY_MAX = 8.f;          // slack of the running maximum, in powers of two (see below)
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
@@ -76,11 +77,12 @@ struct Args {
   float* ml_part;              // [rows * nq, splits, 2]
 };
 
-// Four numbers of a row's output: its sums over the sum of its probabilities, zero where it saw no key.
+// Four numbers of a row's output: its sums over the sum of its probabilities, zero where it saw no key.  (A row that saw keys, all with a
+// score of minus infinity, has sums of zero and a maximum of LOWEST: 0 / 0 is no number.)
 template <typename T>
-__device__ __forceinline__ void write_output(const Args& a, int row, int head, int i, floatx4 sum, float weight) {
+__device__ __forceinline__ void write_output(const Args& a, int row, int head, int i, floatx4 sum, float weight, float most) {
   typedef T vec __attribute__((ext_vector_type(4)));      // (outputs begin at 16 bytes, and their rows)
-  const bool any = weight > 0.f || weight != weight;
+  const bool any = most != NEG_INF;
   const float inv = 1.f / weight;
   vec v;
 #pragma unroll
@@ -214,11 +216,14 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     float p[8];
+    bool some = !MASKED;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = s[i >> 2][qb][i & 3];
-      if (MASKED && !sees(qb, i)) p[i] = NEG_INF;
+      const bool seen = !MASKED || sees(qb, i);
+      some |= seen;
+      p[i] = seen ? s[i >> 2][qb][i & 3] : NEG_INF;
     }
+    r.m[qb] = fmaxf(r.m[qb], some ? LOWEST : NEG_INF);      // (each of the row's lanes for itself)
     float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), p[2]), fmaxf(fmaxf(p[3], p[4]), fmaxf(fmaxf(p[5], p[6]), p[7])));
     if (__any(mx * a.scale2 > r.m[qb] + LAZY_MAX)) {      // some row's maximum grew: rescale what is summed so far
       mx = max_across_rows(mx) * a.scale2;
@@ -229,7 +234,7 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
       for (int db = 0; db < DB; ++db) r.o[qb][db] *= alpha;
       r.m[qb] = m_new;
     }
-    const float neg_m = MASKED && r.m[qb] == NEG_INF ? 0.f : -r.m[qb];      // (no key seen yet: every p is 2^-inf = 0)
+    const float neg_m = -fmaxf(r.m[qb], LOWEST);      // (no score above it yet: every p is 2^-inf = 0)
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = fast_exp2(fmaf(p[i], a.scale2, neg_m));
     r.l[qb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -392,8 +397,9 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
     float l = r.l[qb];
     l += __shfl_xor(l, 16, WAVE);
     l += __shfl_xor(l, 32, WAVE);
+    const float m = max_across_rows(r.m[qb]);
     if (g == 0) {
-      s_m[wave * TR + qb * 16 + c] = r.m[qb];
+      s_m[wave * TR + qb * 16 + c] = m;
       s_l[wave * TR + qb * 16 + c] = l;
     }
 #pragma unroll
@@ -410,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
     float weight = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      // (no maximum: no key that the row sees, sums of zero, or scores that are no numbers, and sums likewise)
+      // (no maximum: no key that the row sees, and sums of zero)
       const float m = s_m[w * TR + row], f = m == NEG_INF ? 1.f : fast_exp2(m - top);
       sum += f * *(const floatx4*)&lds[(w * TR + row) * RS + i];
       weight += f * s_l[w * TR + row];
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
         a.ml_part[(at * a.splits + part) * 2 + 1] = weight;
       }
     } else {
-      write_output<T>(a, r0 + tok, head, i, sum, weight);
+      write_output<T>(a, r0 + tok, head, i, sum, weight, top);
     }
   }
 }
@@ -701,9 +707,15 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
     auto sees = [&](int i) {
       return (there >> (i >> 3) & 1) != 0 && (unsigned)(kb0 + 8 * (i >> 2) + (i & 3) + lane_key) <= span;
     };
+    bool some = true;
     if (masked) {
+      some = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : NEG_INF;
+      for (int i = 0; i < 16; ++i) {
+        const bool seen = sees(i);
+        some |= seen;
+        s[i] = seen ? s[i] : NEG_INF;
+      }
       // (codes that are not numbers: as in add_step)
       bool strange = false;
 #pragma unroll
@@ -739,6 +751,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
         }
       }
     }
+    m = fmaxf(m, some ? LOWEST : NEG_INF);      // (each half of the row's lanes for itself)
     float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
 #pragma unroll
     for (int x = 0; x < 16; x += 2) mx[(x >> 1) & 3] = fmaxf(fmaxf(s[x], s[x + 1]), mx[(x >> 1) & 3]);
@@ -755,7 +768,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
         for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
       m = m_new;
     }
-    const float neg_m = m == NEG_INF ? 0.f : -m;      // (no key seen yet: every p is 2^-inf = 0)
+    const float neg_m = -fmaxf(m, LOWEST);      // (no score above it yet: every p is 2^-inf = 0)
 #pragma unroll
     for (int block = 0; block < 2; ++block) {
       float p[8];
@@ -785,6 +798,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
   __builtin_amdgcn_s_waitcnt(0x0070);      // the last loads (of a tile past the end) are in, and the stages read
   __syncthreads();
   l += __shfl_xor(l, 32, WAVE);
+  m = fmaxf(m, __shfl_xor(m, 32, WAVE));
 
   // (the row's place worked out again: two registers less in the loop)
   int again = row0 + col;
@@ -802,7 +816,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
     if (has_row)
 #pragma unroll
       for (int n = 0; n < DV * 4; ++n)
-        if (place(n) >= 0) write_output<T>(a, r0 + out_tok, out_head, place(n), piece(n), l);
+        if (place(n) >= 0) write_output<T>(a, r0 + out_tok, out_head, place(n), piece(n), l, m);
   } else {
     // group ph puts the pieces ph, ph + P, .. of its rows together; the others' it finds in LDS
     constexpr int SHARES = DV * 4 / P;
@@ -831,7 +845,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      // (no maximum: no key that the row sees, sums of zero, or scores that are no numbers, and sums likewise)
+      // (no maximum: no key that the row sees, and sums of zero)
       w[p] = w[p] == NEG_INF ? 1.f : fast_exp2(w[p] - top);
       weight += w[p] * s_l[(p * RT + rt) * 32 + col];
     }
@@ -842,7 +856,7 @@ __global__ __launch_bounds__(64 * RT * P, staged_waves(parts_of<T>(), P)) void a
       for (int p = 0; p < P; ++p)
         v += w[p] * (p == ph ? mine[n] : left[(((p * RT + rt) * SHARES + n) * (P - 1) + (ph > p ? ph - 1 : ph)) * 64 + lane]);
       const int to = place(n * P + ph);
-      if (has_row && to >= 0) write_output<T>(a, r0 + out_tok, out_head, to, v, weight);
+      if (has_row && to >= 0) write_output<T>(a, r0 + out_tok, out_head, to, v, weight, top);
     }
   }
 }
@@ -905,7 +919,7 @@ __global__ __launch_bounds__(256) void attention_e4m3_merge_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor(sum[j], off, WAVE);
   }
-  if (GROUPS > 1 ? lane < LANES : i < D) write_output<T>(a, row, head, i, sum, l);
+  if (GROUPS > 1 ? lane < LANES : i < D) write_output<T>(a, row, head, i, sum, l, top);
 }
 
 extern "C" const char* llmlab_last_error() { return g_llmlab_error; }

@@ -1248,7 +1248,8 @@ class HipOps:
         ``q_start[b] .. q_start[b + 1] - 1`` of ``q [rows, >= heads * d]`` (one token, a few, or a portion of a prompt;
         none: nothing is done) at the positions from ``start_pos[b]`` on, whose keys and values are already stored; the row at
         position p sees the keys ``max(0, p - window + 1) .. p`` (``window`` None: from 0 on).  Keys whose page the
-        table does not have are not seen, and a row that sees none gives zeros.  ``q`` and ``out [rows, heads * d]`` are
+        table does not have are not seen, and a row that sees none gives zeros (one that sees some, all with scores of minus
+        infinity, numbers that are none).  ``q`` and ``out [rows, heads * d]`` are
         both bfloat16 or both float32 (products in 24 bits); scores, softmax and sums are float32.  ``max_q_len`` and
         ``max_ctx_len`` are the longest portion and context among the requests.  Rows behind the last request keep what they
         hold.  Long contexts of few requests use the kernel set's workspace: calls of one kernel set go to one stream at a time."""
