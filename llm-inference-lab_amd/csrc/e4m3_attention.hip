@@ -1078,6 +1078,8 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
 #endif
   if (dtype == DT_F32)
     return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
-  return most_rows > 16 && D <= 128 ? launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream)
-                                    : launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
+  if constexpr (D <= 128) {      // (above, 32 rows do not fit the registers)
+    if (most_rows > 16) return launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
+  }
+  return launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 }
