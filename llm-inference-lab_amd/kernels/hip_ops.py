@@ -1122,15 +1122,6 @@ class HipOps:
             self.loaded_libraries.append(lib._name)
         return lib
 
-    def check_e4m3_attention_sizes(self, num_heads: int, num_kv_heads: int, head_dim: int, dtype) -> None:
-        if head_dim % 16 != 0 or not 16 <= head_dim <= 256:
-            raise UnsupportedSizeError(f"attention kernels take head sizes that are multiples of 16 from 16 to 256, "
-                                       f"got {head_dim}")
-        if num_heads % num_kv_heads != 0:
-            raise UnsupportedSizeError(f"{num_heads} heads are not a multiple of {num_kv_heads} kv heads")
-        self._e4m3_attention_lib(head_dim)
-        self._mixer_lib("e4m3_cache")
-
     def _e4m3_pages(self, what, k_cache, v_cache, kv_scale, num_kv_heads, head_dim, page_size, block_table):
         """The checks of a cache of 8 bits; its three addresses.  (In one expression first: a call of a decode step is bound by
         what the host does for it, and the checks one by one were a third of that.)"""
