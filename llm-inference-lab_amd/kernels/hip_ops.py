@@ -1277,7 +1277,7 @@ class HipOps:
         reqs, width = block_table.shape
         args = [q_at, kind, q_stride, num_heads, num_kv_heads, keys, values, scales, k_cache.shape[0], block_table.data_ptr(),
                 block_table.stride(0), width, page_size, q_start.data_ptr(), start_pos.data_ptr(), 0, 0, 0,
-                int(window) if window else 0, float(scale), out_at, width_out, rows, self.workspace.data_ptr(),
+                min(int(window), 0x7fffffff) if window else 0, float(scale), out_at, width_out, rows, self.workspace.data_ptr(),
                 self.workspace.numel(), self.num_cus, None]
         return E4m3AttentionCall(self, lib, args,
                                  most_requests=min(q_start.numel() - 1, start_pos.numel(), reqs), most_context=width * page_size)
