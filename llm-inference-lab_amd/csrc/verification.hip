@@ -490,7 +490,7 @@ extern "C" size_t llmlab_verify_drafts_scratch(int n, int rows, int vocab, int w
 extern "C" int llmlab_verify_drafts(const float* logits, size_t stride, const float* draft, size_t draft_stride,
                                     const int* drafts, const int* row_start, const float* temperature, const float* uniform,
                                     int n, int rows, int vocab, int* accepted, int* tokens, void* scratch,
-                                    size_t scratch_bytes, hipStream_t stream) {
+                                    size_t scratch_bytes, int num_cus, hipStream_t stream) {
   LLMLAB_REQUIRE(n >= 0 && rows >= n && vocab > 0, "verify_drafts: bad sizes requests=%d rows=%d vocabulary=%d", n, rows, vocab);
   LLMLAB_REQUIRE(stride >= (size_t)vocab && (draft == nullptr || draft_stride >= (size_t)vocab), "verify_drafts: row strides too small");
   if (n == 0) return 0;
@@ -511,7 +511,7 @@ extern "C" int llmlab_verify_drafts(const float* logits, size_t stride, const fl
   LLMLAB_LAUNCH_CHECK("verify_drafts(chunks)");
   // Two chunks a block once there are more blocks than the chip holds at a time, five a unit: the decision is made half as often
   // (us, one / two, with the draft's logits and without: 32 requests of 152,064 55 / 55 and 38 / 37, 48 77 / 77 and 53 / 48, 64 97 / 93 and 63 / 57).
-  a.each = (long)a.chunks * n > 5 * 256 ? 2 : 1;
+  a.each = (long)a.chunks * n > 5L * (num_cus > 0 ? num_cus : 256) ? 2 : 1;
   hipLaunchKernelGGL(verify_draw_kernel, dim3((a.chunks + a.each - 1) / a.each, n), dim3(THREADS), 0, stream, a);
   LLMLAB_LAUNCH_CHECK("verify_drafts(draw)");
   return 0;

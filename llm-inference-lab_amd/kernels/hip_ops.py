@@ -1391,7 +1391,7 @@ class HipOps:
             if kind == "verification":
                 lib.llmlab_verify_drafts.argtypes = [
                     _c_ptr, _c_size, _c_ptr, _c_size, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr,
-                    _c_ptr, _c_size, _c_ptr]
+                    _c_ptr, _c_size, _c_int, _c_ptr]
                 lib.llmlab_verify_drafts.restype = _c_int
             if kind == "windowed_attention":
                 lib.llmlab_project_norm_write.argtypes = [
@@ -2832,4 +2832,4 @@ class HipOps:
         self._call(lib.llmlab_verify_drafts, self._ptr(logits), logits.stride(0) if rows > 1 else vocab, self._ptr(draft_logits),
                    draft_logits.stride(0) if draft_logits is not None and rows - n > 1 else vocab, self._ptr(drafts),
                    self._ptr(row_start), self._ptr(temperatures), self._ptr(uniforms), n, rows, vocab, self._ptr(accepted),
-                   self._ptr(tokens), self._ptr(self.workspace), self.workspace.numel() * 4, self._stream(), lib=lib)
+                   self._ptr(tokens), self._ptr(self.workspace), self.workspace.numel() * 4, self.num_cus, self._stream(), lib=lib)
