@@ -12,8 +12,9 @@
 // into its probability, in float32 behind the sum of the probabilities.  The numbers of a key are taken in the order in
 // which a lane's 16 bytes hold them (lane group g of a piece of 64: numbers 16 g .. 16 g + 15, the first eight in one
 // product and the others in the next), and the queries alike.  Scores, maxima, exponentials and sums are float32.  A probability
-// times its value's scale is rounded once, to the bfloat16 that the instruction takes (half a step, 2^-9 of itself: outputs 0.0022 off 64
-// bits, 0.0017 of it their own rounding).
+// times its value's scale goes into the product as bfloat16: of rows in one tile of 16 or 32 as two numbers (what is left out is 2^-16 of
+// it, so that the output's own rounding is all that counts: 0.0017 off 64 bits), of more rows rounded once, as in the attention over
+// bfloat16 pages (half a step, up to 2^-8 of itself: outputs 0.0022 off 64 bits).
 //
 // float32 queries are taken as three bfloat16 parts (24 bits: nothing is lost), probabilities too, each part a
 // product of its own; the keys' and values' numbers are exact.
@@ -180,10 +181,10 @@ __device__ __forceinline__ void load_rows(const Args& a, Rows<QB, PARTS>& r, int
   }
 }
 
-// One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  The running
+// One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  P_PARTS: of a probability.  The running
 // maximum is kept in the units of the exponent and is raised only when a score exceeds it by more than LAZY_MAX: until then p may
 // be as large as 2^8, which changes no rounding (bfloat16 has float32's exponents), and rescaling the sums is rare.
-template <bool MASKED, int QB, int PARTS>
+template <bool MASKED, int QB, int PARTS, int P_PARTS>
 __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step& f, int kb, int g) {
   floatx4 s[2][QB];
 #pragma unroll
@@ -212,7 +213,7 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
   }
   auto key = [&](int i) { return kb + (i >> 2) * 16 + g * 4 + (i & 3); };
   auto sees = [&](int qb, int i) { return f.there[i >> 2] && (unsigned)(key(i) - r.lo[qb]) <= r.span[qb]; };
-  bf16x8 pf[QB][PARTS];
+  bf16x8 pf[QB][P_PARTS];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     float p[8];
@@ -240,10 +241,10 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
     r.l[qb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      bf16_t part[PARTS];
-      split<PARTS>(p[i] * vs[i], part);
+      bf16_t part[P_PARTS];
+      split<P_PARTS>(p[i] * vs[i], part);
 #pragma unroll
-      for (int n = 0; n < PARTS; ++n) pf[qb][n][i] = part[n];
+      for (int n = 0; n < P_PARTS; ++n) pf[qb][n][i] = part[n];
     }
   }
   // Places that a row does not see may hold codes that are not numbers, which their probability of zero does not keep
@@ -288,7 +289,7 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-      for (int n = PARTS - 1; n >= 0; --n) r.o[qb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][n], r.o[qb][db], 0, 0, 0);
+      for (int n = P_PARTS - 1; n >= 0; --n) r.o[qb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][n], r.o[qb][db], 0, 0, 0);
   }
 }
 
@@ -307,7 +308,7 @@ constexpr int split_waves(int qb, int parts) {
   if (qb == 1 && parts == 1) return D <= 64 ? 4 : D <= 112 ? 3 : D <= 128 ? 2 : 1;
   return D <= (qb == 2 ? 48 : 64) ? 3 : D <= 128 ? 2 : 1;
 }
-template <typename T, int QB, int NW>
+template <typename T, int QB, int NW, int P_PARTS>
 __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void attention_e4m3_split_kernel(Args a) {
   constexpr int PARTS = parts_of<T>(), TR = 16 * QB, RS = D + 4;
   __shared__ __attribute__((aligned(16))) float lds[split_lds_floats<QB, NW>()];
@@ -385,9 +386,9 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
       __builtin_amdgcn_sched_barrier(0);
       const int kb = step * 32;
       if (cur.there[0] && cur.there[1] && kb + 31 <= first_pos && kb >= full_lo)      // (rows past the last are not stored)
-        add_step<false, QB, PARTS>(a, r, cur, kb, g);
+        add_step<false, QB, PARTS, P_PARTS>(a, r, cur, kb, g);
       else
-        add_step<true, QB, PARTS>(a, r, cur, kb, g);
+        add_step<true, QB, PARTS, P_PARTS>(a, r, cur, kb, g);
     }
   }
 
@@ -949,7 +950,8 @@ static int key_splits(long blocks, int visible, int num_cus) {
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
 // the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (850 others: 0.9 %, 32 % at worst, requests of very different lengths; 500 at heads of
-// 16 to 112, by the figures of 64 or 128, 0.9 %).  Up to 16 rows a
+// 16 to 112, by the figures of 64 or 128, 0.9 %).  Up to 16 rows (32 in
+// bfloat16: one tile, and the estimate is for another form only from thousands of pairs behind 20 keys on) a
 // tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
 // us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
 // of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
@@ -967,8 +969,8 @@ struct Form {
 };
 template <typename T>
 static int launch_form(long most_rows, long pairs, int walk, int visible, int num_cus) {
-  if (most_rows <= 16) return FORM_SPLIT;
   constexpr bool F32 = parts_of<T>() > 1;
+  if (most_rows <= (F32 ? 16 : 32)) return FORM_SPLIT;
   constexpr Form bf16_forms[] = {
       {FORM_SPLIT, 32, SPLIT_WAVES, D <= 64 ? 3.f : 2.f, D <= 64 ? 5.5f : 6.4f, D <= 64 ? 1.14f : 1.18f, D <= 64 ? .54f : .58f, D <= 64 ? .79f : .92f},
       {FORM_2x4, 64, 4, D <= 64 ? 2.f : 1.f, D <= 64 ? 6.f : 8.2f, D <= 64 ? .85f : 1.18f, D <= 64 ? .9f : .34f, D <= 64 ? .83f : 1.f},
@@ -997,7 +999,7 @@ static int launch_form(long most_rows, long pairs, int walk, int visible, int nu
 }
 #endif
 
-template <typename T, int QB>
+template <typename T, int QB, int P_PARTS>
 static int launch_split(Args a, long most_rows, int visible, float* workspace, size_t workspace_floats, int num_cus,
                         hipStream_t stream) {
   const long tiles = (most_rows + 16 * QB - 1) / (16 * QB);
@@ -1009,7 +1011,7 @@ static int launch_split(Args a, long most_rows, int visible, float* workspace, s
     a.o_part = workspace;
     a.ml_part = workspace + (size_t)a.rows * a.nq * a.splits * D;
   }
-  hipLaunchKernelGGL((attention_e4m3_split_kernel<T, QB, SPLIT_WAVES>), dim3((unsigned)tiles, a.nkv * a.splits, a.reqs),
+  hipLaunchKernelGGL((attention_e4m3_split_kernel<T, QB, SPLIT_WAVES, P_PARTS>), dim3((unsigned)tiles, a.nkv * a.splits, a.reqs),
                      dim3(64 * SPLIT_WAVES), 0, stream, a);
   LLMLAB_LAUNCH_CHECK("attention(e4m3)");
   if (a.splits > 1) {
@@ -1061,9 +1063,10 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
   const int visible = window > 0 ? (int)std::min((long)max_ctx_len, (long)window + max_q_len) : max_ctx_len;
   if (num_cus <= 0) num_cus = 256;
+  const bool f32 = dtype == DT_F32;
 #if STAGED
   const int middle = max_ctx_len - max_q_len / 2, walk = window > 0 ? std::min(window, middle) : middle;
-  const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len, f32 = dtype == DT_F32;
+  const bool history = 2L * (max_ctx_len - max_q_len) >= max_q_len;
   // (a cache without pages: nothing there to be read in the place of a missing page.  With no last key the split form walks no step and
   // the rows are zeros; the staged forms read a stage in any case.)
   const int form = pages == 0         ? (int)FORM_SPLIT
@@ -1076,10 +1079,16 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   if (form == FORM_4x1)
     return f32 ? launch_staged<float, 4, 1>(a, most_rows, history, stream) : launch_staged<bf16_t, 4, 1>(a, most_rows, history, stream);
 #endif
-  if (dtype == DT_F32)
-    return launch_split<float, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
-  if constexpr (D <= 128) {      // (above, 32 rows do not fit the registers)
-    if (most_rows > 16) return launch_split<bf16_t, 2>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
+  const auto split = [&](auto launch) { return launch(a, most_rows, visible, workspace, workspace_floats, num_cus, stream); };
+  if (f32) return split(launch_split<float, 1, 3>);
+  // One token or a few, a tile for all their rows: probabilities of two parts, as the reading of the codes bounds them (us, one part / two: 64 tokens of
+  // 28 heads of 128 over 4 at up to 4,096 keys 41.8 / 41.8, of 14 of 64 over 2 15.3 / 15.9, of 8 of 256 over 1 29.4 / 30.5; 8 of 128 at 32,768 44.6 /
+  // 44.8; one of 64 at 700 9.9 / 9.8; 32 requests of 5 tokens of 40 heads over 8 at 2,500 30.1 / 31.6).  More rows: one part, as products bound them
+  // (staged forms: three portions of 1,000 tokens 145 / 192).
+  if (most_rows <= 16) return split(launch_split<bf16_t, 1, 2>);
+  if constexpr (D <= 128) {
+    return most_rows <= 32 ? split(launch_split<bf16_t, 2, 2>) : split(launch_split<bf16_t, 2, 1>);
+  } else {      // (32 rows do not fit the registers)
+    return split(launch_split<bf16_t, 1, 1>);
   }
-  return launch_split<bf16_t, 1>(a, most_rows, visible, workspace, workspace_floats, num_cus, stream);
 }

@@ -15,7 +15,7 @@ WAVES = {"e4m3_staged_kernelIDF16bLi2ELi4E": {16: 4, 80: 2}, "e4m3_staged_kernel
 def test_nothing_is_spilled(d):
     taken = kernels(library(lambda: build.e4m3_attention_library(d)))
     names = [k for k in WAVES if not (d > 128 and ("staged" in k or "Li2E" in k))]
-    assert len(taken) == (10 if d <= 128 else 4)                # (nothing that no call reaches)
+    assert len(taken) == (11 if d <= 128 else 5)                # (nothing that no call reaches)
     for name, (registers, spilled) in taken.items():
         kernel = [k for k in names if k in name]
         assert len(kernel) == 1, name
