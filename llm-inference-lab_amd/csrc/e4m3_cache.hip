@@ -436,8 +436,9 @@ extern "C" int llmlab_rope_kv_write_e4m3(const void* qkv, int dtype, int rows, s
                        row_stride, inv_freq, y, q_stride, rows, a);
   };
   // Many rows: eight a block, a wave each, where their values' codes fit beside the sines; few: four waves a row, so that a row's chain is
-  // short and the rows spread over the chip.  us, few / many: 14 heads of 64 over 2, 1,024 rows 6.1 / 7.4, 2,048 9.4 / 7.8, 8,192
-  // 26.8 / 17.4; 28 of 128 over 4 9.8 / 13.3, 14.5 / 14.1, 46.8 / 37.3; 64 of 128 over 8 14.0 / 23.2, 21.3 / 24.3, 78 / 77.  (Sixteen rows a block:
+  // short and the rows spread over the chip.  us of GPU, few / many: 14 heads of 64 over 2, 1,024 rows 5.7 / 6.9, 2,048 9.0 / 7.4, 8,192
+  // 25.7 / 16.7; 28 of 128 over 4 9.2 / 12.9, 14.2 / 14.5, 48.8 / 38.1; 64 of 128 over 8 14.0 / 23.2, 21.3 / 24.3, 78 / 77.  float32: 14 of 64 over 2
+  // 5.8 / 6.8, 9.5 / 8.2, 25.8 / 16.8; 28 of 128 over 4 9.5 / 12.6, 14.8 / 16.2, 57.2 / 61.0 (the one kind that loses a little).  (Sixteen rows a block:
   // 2,048 rows 19.2, 8,192 37.8; four: 13.8 and 40.1; two waves a row 13.2 and 45.8; all waves of a block over its rows one
   // after the other 20.8 and 45.4.)
   constexpr int MANY = 8;
@@ -467,8 +468,10 @@ extern "C" int llmlab_read_kv_e4m3(const void* k, const void* v, const void* sca
   if (rc) return rc;
   if (rows == 0) return 0;
   LLMLAB_REQUIRE((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "read_kv_e4m3: the outputs are not aligned to 16 bytes");
-  // Four rows a wave once the rows fill the chip so (us, four / one, 8 heads of 128: 2,048 rows in order 10.8 / 8.5, 8,192 14.8 / 14.2, 16,384
-  // 19.1 / 31.2; in any order 18.7 / 9.7, 23.7 / 19.1, 33.4 / 38.2).
+  // Four rows a wave once the rows fill the chip so, whatever their width (us of GPU, one / four.  bfloat16, 8 heads of 128: 2,048 rows in order
+  // 8.2 / 10.5, 8,192 14.2 / 13.9, 16,384 30.5 / 19.6, 32,768 59.1 / 37.5; in any order 10.1 / 19.3, 23.9 / 27.0, 45.9 / 38.4, 82.9 / 83.3: there
+  // a lane's 16 bytes of values have four of its own, and four of four rows in order.  2 heads of 64: 8,192 6.9 / 6.9 and in any order
+  // 7.7 / 9.7, 16,384 11.7 / 8.3 and 12.1 / 11.5.  float32, 8 of 128: 8,192 22.6 / 21.2 and 31.6 / 35.6, 16,384 47.4 / 33.6 and 61.9 / 51.2).
   auto pick = [&](auto t) {
     typedef decltype(t) T;
     if (rows > 8192)

@@ -47,7 +47,9 @@ struct VerifyArgs {
 // n by adding 1.5 * 2^52 (its low word then is n), the polynomial of degree 8 that meets 2^f at the nine Chebyshev points of
 // [-1/2, 1/2] (zero among them), and n added to the exponent's bits.  Below 2^-1023 it is zero: f is zero there, the polynomial 1 and
 // its exponent's bits all gone.  (Every step at the rate of a product: a rint, a conversion and an ldexp are slower, and the
-// exponentials bound the first launch.)
+// exponentials bound the first launch.)  1.1e-12 is enough: one of 150,000 borders between tokens lies so near a given random number once in
+// six million draws.  Degree 10 (3e-16, full 64 bits) takes 100 us where this takes 94 (64 requests, five drafts each with logits, 152,064
+// tokens), 61 and 57 without.
 __device__ __forceinline__ double exp2_below(double y) {
   constexpr double WHOLE = 6755399441055744.0;
   y = fmax(y, -1023.0);
