@@ -296,8 +296,8 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 // Few rows a request: NW waves share a tile of 16 QB rows (a row: a token and a head of the group that shares a kv head) and
 // split the block's keys in steps of 32; their sums meet in LDS.  The keys of a tile are split over a.splits blocks as
 // well, whose sums a kernel of its own puts together.  Bound by the reading of the codes where a request brings a token or a few: 64 requests
-// of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 40 and 4.7 of the merge; 32 of
-// 5 tokens of 40 heads over 8 at 2,500 (124 MB) 30.  float32 rows by their products, three a part: 7 of 61 tokens of 16 heads over 2 through a
+// of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 40 and 4.6 of the merge; 32 of
+// 5 tokens of 40 heads over 8 at 2,500 (124 MB) 31.5 (30 with probabilities of one part).  float32 rows by their products, three a part: 7 of 61 tokens of 16 heads over 2 through a
 // window of 1,000 22 us.
 template <int QB, int NW>
 constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
@@ -453,8 +453,8 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 //
 // What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
 // instructions (512 clocks of a SIMD) and some 170 others (680 and more), 64 of them conversions; three portions of 1,000 tokens behind
-// up to 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 149 to 159 us (0.76 to 0.81 PFLOP/s), 62 % of the clocks in vector and 35 % in
-// matrix instructions, a sixth without a block.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
+// up to 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 145 to 148 us (0.82 to 0.83 PFLOP/s), 62 % of the clocks in vector and 36 % in
+// matrix instructions, a sixth without a block.  A probability is one bfloat16 number: two take 192 us.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
 // loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
 // 2^-16 of the sum of sizes), so not used.  float32 rows take three products a part of what they read, and as many conversions of codes as one:
 // 7 requests of 700 tokens, 56 heads of 128 over 8, up to 1,400 keys 273 us (split over waves 439).

@@ -1241,7 +1241,8 @@ class HipOps:
         position p sees the keys ``max(0, p - window + 1) .. p`` (``window`` None: from 0 on).  Keys whose page the
         table does not have are not seen, and a row that sees none gives zeros (one that sees some, all with scores of minus
         infinity, numbers that are none).  ``q`` and ``out [rows, heads * d]`` are
-        both bfloat16 or both float32 (products in 24 bits); scores, softmax and sums are float32.  ``max_q_len`` and
+        both bfloat16 or both float32 (products in 24 bits); scores, softmax and sums are float32.  bfloat16 rows of a token or a
+        few (up to 32 a kv head) are as exact as their output's rounding; of more, each probability is rounded to bfloat16 too.  ``max_q_len`` and
         ``max_ctx_len`` are the longest portion and context among the requests.  Rows behind the last request keep what they
         hold.  Long contexts of few requests use the kernel set's workspace: calls of one kernel set go to one stream at a time."""
         self.prepare_attention_e4m3(q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, kv_scale, block_table, page_size,
@@ -2805,7 +2806,7 @@ class HipOps:
         last row's ``p``: the first token at which the running sum reaches ``uniforms[row_start[b + 1] - 1]`` times
         the whole.  Temperature 0: a token stands while it is its row's argmax (the smallest index among equals), and the
         next token is the argmax of the row that is reached.  ``accepted[b]`` is how many stand, ``tokens[b]`` the
-        next token, -1 where its row is no distribution.  A logit that is not a number counts as minus infinity, a drafted
+        next token, -1 where its row (or the draft's of the token that fell) is no distribution.  A logit that is not a number counts as minus infinity, a drafted
         token outside the vocabulary falls.  ``uniforms [rows]`` are in [0, 1).  The kernel set's workspace is used:
         calls of one kernel set go to one stream at a time."""
         what = "verify_drafts"
