@@ -181,8 +181,8 @@ __device__ __forceinline__ void load_rows(const Args& a, Rows<QB, PARTS>& r, int
   }
 }
 
-// One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  P_PARTS: of a probability.  The running
-// maximum is kept in the units of the exponent and is raised only when a score exceeds it by more than LAZY_MAX: until then p may
+// One step of 32 keys from kb on for every row of the tile.  MASKED: some row does not see some key.  P_PARTS: the bfloat16 numbers
+// that a probability is taken as.  The running maximum is kept in the units of the exponent and is raised only when a score exceeds it by more than LAZY_MAX: until then p may
 // be as large as 2^8, which changes no rounding (bfloat16 has float32's exponents), and rescaling the sums is rare.
 template <bool MASKED, int QB, int PARTS, int P_PARTS>
 __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step& f, int kb, int g) {
@@ -297,8 +297,8 @@ __device__ __forceinline__ void add_step(const Args& a, Rows<QB, PARTS>& r, Step
 // split the block's keys in steps of 32; their sums meet in LDS.  The keys of a tile are split over a.splits blocks as
 // well, whose sums a kernel of its own puts together.  Bound by the reading of the codes where a request brings a token or a few: 64 requests
 // of 28 heads of 128 over 4 at up to 4,096 keys (197 MB) 42 us of kernel (4.7 TB/s), 8 at 32,768 40 and 4.6 of the merge; 32 of
-// 5 tokens of 40 heads over 8 at 2,500 (124 MB) 31.5 (30 with probabilities of one part).  float32 rows by their products, three a part: 7 of 61 tokens of 16 heads over 2 through a
-// window of 1,000 22 us.
+// 5 tokens of 40 heads over 8 at 2,500 (124 MB) 31.5 (30 with probabilities of one part).  float32 rows by their products, three a part:
+// 7 of 61 tokens of 16 heads over 2 through a window of 1,000 22 us.
 template <int QB, int NW>
 constexpr int split_lds_floats() { return NW * 16 * QB * (D + 4) + 2 * NW * 16 * QB; }
 
@@ -454,8 +454,9 @@ __global__ __launch_bounds__(64 * NW, split_waves(QB, parts_of<T>())) void atten
 // What bounds it: the vector unit beside the matrix cores.  A step of a wave, 32 keys by 32 rows at heads of 128, is 16 matrix
 // instructions (512 clocks of a SIMD) and some 170 others (680 and more), 64 of them conversions; three portions of 1,000 tokens behind
 // up to 3,000 keys (28 heads of 128 over 4, 121 GFLOP) take 145 to 148 us (0.82 to 0.83 PFLOP/s), 62 % of the clocks in vector and 36 % in
-// matrix instructions, a sixth without a block.  A probability is one bfloat16 number: two take 192 us.  Numbers made bfloat16 on the way into LDS, once for a block: slower (366 us, its
-// loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
+// matrix instructions, a sixth without a block.  A probability is one bfloat16 number: two take 192 us, one of half precision in units of
+// the largest value's scale 152 to 154 and a second path where scales differ much.  Numbers made bfloat16 on the way into LDS, once for a
+// block: slower (366 us, its loads through registers).  Products in 8 bits, with the queries as two parts: exact products, but sums kept to 16 bits (measured:
 // 2^-16 of the sum of sizes), so not used.  float32 rows take three products a part of what they read, and as many conversions of codes as one:
 // 7 requests of 700 tokens, 56 heads of 128 over 8, up to 1,400 keys 273 us (split over waves 439).
 #define STAGED (HEAD_DIM <= 128)
@@ -950,9 +951,9 @@ static int key_splits(long blocks, int visible, int num_cus) {
 // its steps of 32 keys x a step), in us as fitted to 800 launches drawn at random (1 to 64 requests of 1 to 2,048 tokens
 // behind 0 to 32,768 keys, of one length and of different ones, eight head layouts, a quarter through windows), over which
 // the picks lose 0.3 % (heads of 64) and 0.5 % (128) to the best of all (850 others: 0.9 %, 32 % at worst, requests of very different lengths; 500 at heads of
-// 16 to 112, by the figures of 64 or 128, 0.9 %).  Up to 16 rows (32 in
-// bfloat16: one tile, and the estimate is for another form only from thousands of pairs behind 20 keys on) a
-// tile's keys are split over waves and blocks; of more rows so, too, where they are few or the keys many.
+// 16 to 112, by the figures of 64 or 128, 0.9 %).  Up to 16 rows (32 in bfloat16: one tile; the estimate takes another form there only for
+// thousands of pairs behind some 20 keys) a tile's keys are split over waves and blocks; of more rows so, too, where they are few or the
+// keys many.
 // us, split / 2x4 / 2x2 / 4x1, heads of 128: 35 rows of 72 (request, kv head) pairs behind 6,652 keys 47 / 68 / 89 / 165; 152
 // of 72 behind 2,380 44 / 34 / 39.5 / 66; 640 of 68 behind 229 31 / 33 / 20.6 / 24.7; 10,829 of 8 and 1,547 keys 91 / 89 / 58 / 58;
 // 1,304 of 40 behind 63 32 / 38 / 26 / 21.5; 6,624 of 48 behind 232 241 / 269 / 161 / 148.
@@ -1057,8 +1058,8 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
   if (reqs == 0 || max_q_len <= 0 || rows == 0) return 0;
   Args a{q, (const unsigned char*)k, (const unsigned char*)v, (const unsigned char*)kv_scale, table, q_start, start_pos, out,
          q_stride, out_stride, table_stride, table_width, 0, pages,
-         pages == 0 ? -1 : (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, 0, scale * 1.4426950408889634f,
-         nullptr, nullptr};
+         pages == 0 ? -1 : (int)std::min((long)table_width * page_size, 0x7fffffffL) - 1, nq, nkv, window, rows, reqs, 1, 0,
+         scale * 1.4426950408889634f, nullptr, nullptr};
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   const long most_rows = (long)std::min(max_q_len, rows) * (nq / nkv);
   const int visible = window > 0 ? (int)std::min((long)max_ctx_len, (long)window + max_q_len) : max_ctx_len;
@@ -1081,10 +1082,10 @@ extern "C" int llmlab_paged_attention_e4m3(const void* q, int dtype, long q_stri
 #endif
   const auto split = [&](auto launch) { return launch(a, most_rows, visible, workspace, workspace_floats, num_cus, stream); };
   if (f32) return split(launch_split<float, 1, 3>);
-  // One token or a few, a tile for all their rows: probabilities of two parts, as the reading of the codes bounds them (us, one part / two: 64 tokens of
-  // 28 heads of 128 over 4 at up to 4,096 keys 41.8 / 41.8, of 14 of 64 over 2 15.3 / 15.9, of 8 of 256 over 1 29.4 / 30.5; 8 of 128 at 32,768 44.6 /
-  // 44.8; one of 64 at 700 9.9 / 9.8; 32 requests of 5 tokens of 40 heads over 8 at 2,500 30.1 / 31.6).  More rows: one part, as products bound them
-  // (staged forms: three portions of 1,000 tokens 145 / 192).
+  // One token or a few, a tile for all their rows: probabilities of two parts, as the reading of the codes bounds them (us, one part /
+  // two: 64 tokens of 28 heads of 128 over 4 at up to 4,096 keys 41.8 / 41.8, of 14 of 64 over 2 15.3 / 15.9, of 8 of 256 over 1 29.4 /
+  // 30.5; 8 of 128 at 32,768 44.6 / 44.8; one of 64 at 700 9.9 / 9.8; 32 requests of 5 tokens of 40 heads over 8 at 2,500 30.1 / 31.6).
+  // More rows: one part, as products bound them (staged forms: three portions of 1,000 tokens 145 / 192).
   if (most_rows <= 16) return split(launch_split<bf16_t, 1, 2>);
   if constexpr (D <= 128) {
     return most_rows <= 32 ? split(launch_split<bf16_t, 2, 2>) : split(launch_split<bf16_t, 2, 1>);
