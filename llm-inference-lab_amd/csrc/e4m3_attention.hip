@@ -941,7 +941,7 @@ constexpr int SPLIT_WAVES = 4;
 // up to 32 steps, where the launch that puts the splits together costs what they gain (one to 16 requests of 28 heads of 128 over 4 at 700
 // to 1,000 keys 7.9 to 10.3 us of GPU in one launch, 8.1 to 10.3 in two, and the host 2.8 us less; at 1,500 11.4 and 8.4).
 static int key_splits(long blocks, int visible, int num_cus) {
-  const long steps = (visible + 31) / 32, most = (steps + 7) / 8;
+  const long steps = (visible + 31L) / 32, most = (steps + 7) / 8;
   if (blocks >= num_cus || steps <= 32) return 1;
   return (int)std::max(1L, std::min(std::min(2L * num_cus / blocks, most), 128L));
 }
