@@ -194,8 +194,9 @@ class E4m3AttentionCall:
         if max_ctx_len > self.most_context:
             raise ValueError("attention: the block table is too narrow for the longest context")
         a = self.args
-        most = 0x7fffffff        # (a 32-bit argument would take the low bits alone of a longer bound)
-        a[self.REQS], a[self.MAX_Q], a[self.MAX_CTX] = n_reqs, min(max_q_len, most), min(max_ctx_len, most)
+        a[self.REQS], a[self.MAX_Q], a[self.MAX_CTX] = n_reqs, max_q_len, max_ctx_len
+        if max_q_len > 0x7fffffff or max_ctx_len > 0x7fffffff:      # (a 32-bit argument would take the low bits alone)
+            a[self.MAX_Q], a[self.MAX_CTX] = min(max_q_len, 0x7fffffff), min(max_ctx_len, 0x7fffffff)
         a[self.STREAM] = self.ops._stream()
         self.ops._call(self.lib.llmlab_paged_attention_e4m3, *a, lib=self.lib)
 
